@@ -76,6 +76,12 @@ SIGNATURES = {
     "cf_reci_phase": [P, P, P, P, I64, P, P],
     "cf_reci_sum_fwd": [P, P, P, P, P, P, I64, I64, I64, I32, P, P, P],
     "cf_reci_sum_bwd": [P, P, P, P, P, P, P, I64, I64, I64, I32, P, P],
+    "cf_embed_fwd": [P, I64, I64, I32, P, I64, I64, I64, F64, P, P],
+    "cf_embed_bwd_workspace_bytes": [I64, I64],
+    "cf_embed_bwd": [P, I64, I32, P, I64, I64, I64, F64, P, I32, P, P],
+    "cf_qk_norm_fwd": [P, P, P, P],
+    "cf_qk_norm_bwd_workspace_bytes": [P],
+    "cf_qk_norm_bwd": [P, P, P, P, P, P, P, P, P],
     "cf_encoder_forward": [P, I32, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, F64, F64, I32, I32, P, P, P,
                            P],
 }
@@ -131,6 +137,14 @@ class ServeGather(ctypes.Structure):
                 ("timeout_s", c_double)]
 
 
+class QkNorm(ctypes.Structure):
+    """``cf_qk_norm``: the arguments of the norms and rotation of queries and keys."""
+    _fields_ = [("type", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("N", c_int64), ("Hq", c_int64), ("Hk", c_int64), ("D", c_int64),
+                ("P", c_int64), ("C", c_int64), ("wave_heads", c_int64), ("q", c_void_p), ("q_row", c_int64), ("q_head", c_int64),
+                ("k", c_void_p), ("k_row", c_int64), ("k_head", c_int64), ("wq", c_void_p), ("wq_head", c_int64), ("wk", c_void_p),
+                ("wk_head", c_int64), ("pos", c_void_p), ("waves", c_void_p), ("eps", c_double)]
+
+
 class CrystalformerB200Error(RuntimeError):
     """A C-ABI call returned a negative status."""
 
@@ -173,7 +187,7 @@ def load() -> ctypes.CDLL:
             fn.argtypes = argtypes
             fn.restype = c_int
         for name in ("cf_model_head_floats", "cf_lattice_sum_bwd_proj_floats", "cf_dense_image_bytes", "cf_train_saved_bytes", "cf_train_edge_bytes",
-                     "cf_train_scratch_bytes"):
+                     "cf_train_scratch_bytes", "cf_embed_bwd_workspace_bytes", "cf_qk_norm_bwd_workspace_bytes"):
             getattr(lib, name).restype = c_int64
         _lib = lib
     return _lib

@@ -6,7 +6,7 @@ fused attention module; they have no CPU path.
 """
 from __future__ import annotations
 
-from ctypes import c_double, c_int, c_int64, c_void_p
+from ctypes import byref, c_double, c_int, c_int64, c_void_p
 from typing import Optional, Tuple
 
 import torch
@@ -538,3 +538,139 @@ def pipe_probe(kind: int, blocks: int, threads: int, iters: int, sink: torch.Ten
     with torch.cuda.device(sink.device):
         _lib.call("cf_pipe_probe", c_int(kind), c_int(blocks), c_int(threads), c_int64(iters), _ptr(sink),
                   _stream(sink.device))
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Operators of an encoder layer beside the attention, in float32, bfloat16 and float16 (inputs and outputs of one type)
+# ---------------------------------------------------------------------------------------------------------------------
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # CF_FLOAT32, CF_BFLOAT16, CF_FLOAT16
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """The call with `device` current and its current stream as the last argument."""
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _like(t: Optional[torch.Tensor], first: torch.Tensor, name: str, shape) -> None:
+    """Checks that `t` is there, lies where `first` does, with its type and the shape given."""
+    if t is None:
+        return
+    if t.device != first.device:
+        raise RuntimeError(f"{name} is on {t.device}, expected {first.device}")
+    if t.dtype != first.dtype:
+        raise TypeError(f"{name} must be {first.dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _first(t: torch.Tensor, name: str, dims: int) -> torch.Tensor:
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor: crystalformer_b200 has no CPU path")
+    if t.dtype not in TYPE_CODES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got the shape {tuple(t.shape)}")
+    return t
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t, copied unless the entries of its rows are neighbours."""
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 and t.is_contiguous() else t.contiguous()
+
+
+def _ids(ids: torch.Tensor, device) -> torch.Tensor:
+    if ids.device != device:
+        raise RuntimeError(f"ids are on {ids.device}, expected {device}")
+    if ids.dtype != torch.int64:
+        if ids.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+            raise TypeError(f"ids must be whole numbers, got {ids.dtype}")
+        ids = ids.to(torch.int64)
+    return ids if ids.is_contiguous() else ids.contiguous()
+
+
+def embed_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[ids], (*ids.shape, D); ids outside the table give rows of zeros.  ``table`` (V,D) may have any strides."""
+    table = _first(table, "table", 2)
+    ids = _ids(ids, table.device)
+    V, D = table.shape
+    out = torch.empty((*ids.shape, D), dtype=table.dtype, device=table.device)
+    _call_on(table.device, "cf_embed_fwd", table.data_ptr(), table.stride(0), table.stride(1), TYPE_CODES[table.dtype], ids.data_ptr(), ids.numel(),
+             V, D, scale, out.data_ptr())
+    return out
+
+
+def embed_bwd(ids: torch.Tensor, gout: torch.Tensor, V: int, scale: float = 1.0, transposed: bool = False) -> torch.Tensor:
+    """The gradient (V,D) of the table of ``embed_fwd`` from that of its output; ``transposed``: a view of a (D,V) contiguous tensor."""
+    if not gout.is_cuda:
+        raise RuntimeError("gout must be a CUDA tensor: crystalformer_b200 has no CPU path")
+    dev, D = gout.device, gout.shape[-1]
+    ids = _ids(ids, dev)
+    if tuple(gout.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"gout {tuple(gout.shape)} does not belong to ids {tuple(ids.shape)}")
+    gout = _first(gout.reshape(-1, D), "gout", 2)
+    gout = _rows(gout)
+    N = ids.numel()
+    gtable = torch.empty((D, V) if transposed else (V, D), dtype=gout.dtype, device=dev)
+    work = torch.empty(int(_lib.load().cf_embed_bwd_workspace_bytes(N, D)), dtype=torch.uint8, device=dev)
+    _call_on(dev, "cf_embed_bwd", gout.data_ptr(), gout.stride(0) if N > 1 else D, TYPE_CODES[gout.dtype], ids.data_ptr(), N, V, D, scale,
+             gtable.data_ptr(), int(transposed), work.data_ptr())
+    return gtable.t() if transposed else gtable
+
+
+def _qk_args(q, k, wq, wk, pos, waves, eps: float, interleaved: bool):
+    """The description of a call, and the tensors that it points into."""
+    q, k = _first(q, "q", 3), _first(k, "k", 3)
+    N, Hq, D = q.shape
+    Hk = k.shape[1]
+    _like(k, q, "k", (N, Hk, D))
+    q, k = _rows(q), _rows(k)
+    heads = []
+    for name, w, H in (("wq", wq, Hq), ("wk", wk, Hk)):
+        _like(w, q, name, (H, D) if w is not None and w.dim() == 2 else (D,))
+        heads.append(None if w is None else w.contiguous())
+    wq, wk = heads
+    P = C = 0
+    wave_heads = 1
+    if waves is not None:
+        if waves.dim() != 3 or pos is None or pos.dim() != 2 or pos.shape != (N, waves.shape[2]):
+            raise ValueError(f"waves (heads, pairs, axes) and pos (rows, axes) go together: got {tuple(waves.shape)} and "
+                             f"{None if pos is None else tuple(pos.shape)} for {N} rows")
+        pos, waves = _want(pos, torch.float32, "pos", q.device), _want(waves, torch.float32, "waves", q.device)
+        wave_heads, P, C = waves.shape
+    elif pos is not None:
+        raise ValueError("positions without waves")
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    args = _lib.QkNorm(TYPE_CODES[q.dtype], int(interleaved), N, Hq, Hk, D, P, C, wave_heads, ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0),
+                       k.stride(1), ptr(wq), D if wq is not None and wq.dim() == 2 else 0, ptr(wk), D if wk is not None and wk.dim() == 2 else 0,
+                       ptr(pos), ptr(waves), eps)
+    return args, (q, k, wq, wk, pos, waves)
+
+
+def qk_norm_fwd(q, k, wq=None, wk=None, pos=None, waves=None, eps: float = 1e-6, interleaved: bool = False):
+    """Norms of the heads of q (N,Hq,D) and k (N,Hk,D), times the weights, then the rotation by positions (cf_qk_norm_fwd)."""
+    args, keep = _qk_args(q, k, wq, wk, pos, waves, eps, interleaved)
+    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in keep[:2])
+    _call_on(q.device, "cf_qk_norm_fwd", byref(args), q_out.data_ptr(), k_out.data_ptr())
+    return q_out, k_out
+
+
+def qk_norm_bwd(q, k, wq, wk, pos, waves, eps: float, interleaved: bool, gq_out, gk_out, want_wq: bool = True, want_wk: bool = True):
+    """Gradients (gq, gk, gwq, gwk) of ``qk_norm_fwd``'s inputs; those of absent or unwanted weights are None."""
+    args, keep = _qk_args(q, k, wq, wk, pos, waves, eps, interleaved)
+    _like(gq_out, q, "gq_out", q.shape)
+    _like(gk_out, q, "gk_out", k.shape)
+    gq_out, gk_out = gq_out.contiguous(), gk_out.contiguous()
+    dev = q.device
+    gq, gk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in keep[:2])
+    gwq, gwk = (None if w is None or not want else torch.empty(w.shape, dtype=w.dtype, device=dev) for w, want in ((wq, want_wq), (wk, want_wk)))
+    work = None
+    if gwq is not None or gwk is not None:
+        with torch.cuda.device(dev):
+            work = torch.empty(int(_lib.load().cf_qk_norm_bwd_workspace_bytes(byref(args))), dtype=torch.uint8, device=dev)
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    _call_on(dev, "cf_qk_norm_bwd", byref(args), gq_out.data_ptr(), gk_out.data_ptr(), gq.data_ptr(), gk.data_ptr(), ptr(gwq), ptr(gwk), ptr(work))
+    return gq, gk, gwq, gwk

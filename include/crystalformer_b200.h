@@ -658,6 +658,56 @@ int cf_wait_probe(int64_t limit_ns, void *stream);
  * ---------------------------------------------------------------------------------------------------------- */
 int cf_pipe_probe(int kind, int blocks, int threads, int64_t iters, float *sink, void *stream);
 
+/* ------------------------------------------------------------------------------------------------------------
+ * Operators of an encoder layer beside the attention, in three storage types.  Inputs, outputs and gradients have the type of
+ * the call; sums, norms and angles are float32, rounded once.  No counterpart in the reference (its model multiplies one-hot
+ * species by a Linear weight, models/latticeformer.py:224, has no norms of queries and keys, and a ReLU feed-forward,
+ * models/indexed_latticeformer_encoder.py:884-890).
+ * ---------------------------------------------------------------------------------------------------------- */
+#define CF_FLOAT32 0
+#define CF_BFLOAT16 1
+#define CF_FLOAT16 2
+
+/* Embedding lookup with scaling: out (N,D) = scale * table[ids]; an id outside [0, V) (padding) gives a row of zeros.  table
+ * (V,D) by strides in values, so that the transposed weight of a Linear is read where it lies.
+ * Backward: gtable[v] = scale * the sum of the rows of gout (row stride ld) whose id is v, in the rows' order, the same bits
+ * every time; all of gtable is written, (V,D) contiguous or, transposed != 0, (D,V) contiguous.
+ * workspace: cf_embed_bwd_workspace_bytes(N, D) bytes, 16-byte aligned.  N, V <= 2^30, D <= 65536. */
+#define CF_EMBED_MAX_ROWS (1ll << 30)
+int cf_embed_fwd(const void *table, int64_t row_stride, int64_t col_stride, int type, const int64_t *ids, int64_t N,
+                 int64_t V, int64_t D, double scale, void *out, void *stream);
+int64_t cf_embed_bwd_workspace_bytes(int64_t N, int64_t D);
+int cf_embed_bwd(const void *gout, int64_t ld, int type, const int64_t *ids, int64_t N, int64_t V, int64_t D, double scale,
+                 void *gtable, int transposed, void *workspace, void *stream);
+
+/* Root-mean-square norms of the query and key heads, then the rotation by positions:
+ *   y = w x / sqrt(mean x^2 + eps);  theta_p = 2 pi sum_c pos[n,c] waves[h,p,c];  (y1, y2) -> (y1 cos - y2 sin, y1 sin + y2 cos)
+ * for P pairs of entries (p, P + p), interleaved: (2p, 2p + 1); entries from 2 P on are not rotated (P = 0: norms only).
+ * q (N,Hq,D), k (N,Hk,D) by strides in values, entries of a head contiguous; Hq a multiple of Hk, query head h goes with key
+ * head h / (Hq / Hk).  Weights NULL, (D) (head stride 0) or (H,D) (head stride D).  pos (N,C) and waves (wave_heads,P,C)
+ * float32, C <= 3, wave_heads 1 or Hk; waves in cycles per unit of position, their products with positions taken exactly.
+ * D <= CF_QK_NORM_MAX_DIM.  Outputs and gradients of inputs are contiguous; gwq, gwk may be NULL.  Positions and waves have no
+ * gradient.  workspace: cf_qk_norm_bwd_workspace_bytes(args) bytes (of the device that is current), 16-byte aligned. */
+#define CF_QK_NORM_MAX_DIM 512
+typedef struct cf_qk_norm {
+    int32_t type, interleaved;
+    int64_t N, Hq, Hk, D, P, C, wave_heads;
+    const void *q;
+    int64_t q_row, q_head;
+    const void *k;
+    int64_t k_row, k_head;
+    const void *wq;
+    int64_t wq_head;
+    const void *wk;
+    int64_t wk_head;
+    const float *pos, *waves;
+    double eps;
+} cf_qk_norm;
+int cf_qk_norm_fwd(const cf_qk_norm *args, void *q_out, void *k_out, void *stream);
+int64_t cf_qk_norm_bwd_workspace_bytes(const cf_qk_norm *args);
+int cf_qk_norm_bwd(const cf_qk_norm *args, const void *gq_out, const void *gk_out, void *gq, void *gk, void *gwq, void *gwk,
+                   void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
