@@ -82,6 +82,9 @@ SIGNATURES = {
     "cf_qk_norm_fwd": [P, P, P, P],
     "cf_qk_norm_bwd_workspace_bytes": [P],
     "cf_qk_norm_bwd": [P, P, P, P, P, P, P, P, P],
+    "cf_gated_ffn_workspace_bytes": [P, P, I32],
+    "cf_gated_ffn_fwd": [P, P, P, P],
+    "cf_gated_ffn_bwd": [P, P, P, P],
     "cf_encoder_forward": [P, I32, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, F64, F64, I32, I32, P, P, P,
                            P],
 }
@@ -145,6 +148,18 @@ class QkNorm(ctypes.Structure):
                 ("wk_head", c_int64), ("pos", c_void_p), ("waves", c_void_p), ("eps", c_double)]
 
 
+class GatedFFN(ctypes.Structure):
+    """``cf_gated_ffn``: the arguments of the gated feed-forward block."""
+    _fields_ = [("type", ctypes.c_int32), ("activation", ctypes.c_int32), ("N", c_int64), ("D", c_int64), ("F", c_int64), ("x", c_void_p),
+                ("ldx", c_int64), ("w_gate", c_void_p), ("w_up", c_void_p), ("w_down", c_void_p), ("b_gate", c_void_p), ("b_up", c_void_p),
+                ("b_down", c_void_p)]
+
+
+class GatedFFNGrads(ctypes.Structure):
+    """``cf_gated_ffn_grads``: the output's gradient, and where those of the arguments go (None: not wanted)."""
+    _fields_ = [(n, c_void_p) for n in ("gy", "x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down")]
+
+
 class CrystalformerB200Error(RuntimeError):
     """A C-ABI call returned a negative status."""
 
@@ -187,7 +202,8 @@ def load() -> ctypes.CDLL:
             fn.argtypes = argtypes
             fn.restype = c_int
         for name in ("cf_model_head_floats", "cf_lattice_sum_bwd_proj_floats", "cf_dense_image_bytes", "cf_train_saved_bytes", "cf_train_edge_bytes",
-                     "cf_train_scratch_bytes", "cf_embed_bwd_workspace_bytes", "cf_qk_norm_bwd_workspace_bytes"):
+                     "cf_train_scratch_bytes", "cf_embed_bwd_workspace_bytes", "cf_qk_norm_bwd_workspace_bytes",
+                     "cf_gated_ffn_workspace_bytes"):
             getattr(lib, name).restype = c_int64
         _lib = lib
     return _lib

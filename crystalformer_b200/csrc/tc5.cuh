@@ -68,6 +68,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
                  "r"(bytes), "r"(bar)
                  : "memory");
 }
+// box of a tensor map (a kernel parameter, __grid_constant__) -> shared; x: the innermost coordinate, on 16 bytes
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
 // ordinary shared-memory writes of this thread become visible to tcgen05.mma (the asynchronous proxy)
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -99,6 +106,32 @@ __device__ __forceinline__ void tmem_load_16x32(uint32_t addr, float (&v)[16])
         : "memory");  // (load and wait in one statement: the registers are valid when it ends)
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// 32 lanes (the warp's quarter of the 128) x 16 columns: lane l has row l.  Of COUNT accumulators at once, `apart` columns apart.
+template <int COUNT>
+__device__ __forceinline__ void tmem_load_rows16(uint32_t addr, uint32_t apart, float (&v)[COUNT][16])
+{
+    uint32_t r[COUNT][16];
+#pragma unroll
+    for (int c = 0; c < COUNT; ++c)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(r[c][0]), "=r"(r[c][1]), "=r"(r[c][2]), "=r"(r[c][3]), "=r"(r[c][4]), "=r"(r[c][5]), "=r"(r[c][6]), "=r"(r[c][7]),
+                       "=r"(r[c][8]), "=r"(r[c][9]), "=r"(r[c][10]), "=r"(r[c][11]), "=r"(r[c][12]), "=r"(r[c][13]), "=r"(r[c][14]), "=r"(r[c][15])
+                     : "r"(addr + (uint32_t)c * apart)
+                     : "memory");
+    // (the registers pass through the wait, so that nothing reads them before it)
+#pragma unroll
+    for (int c = 0; c < COUNT; ++c)
+        asm volatile("tcgen05.wait::ld.sync.aligned;"
+                     : "+r"(r[c][0]), "+r"(r[c][1]), "+r"(r[c][2]), "+r"(r[c][3]), "+r"(r[c][4]), "+r"(r[c][5]), "+r"(r[c][6]), "+r"(r[c][7]),
+                       "+r"(r[c][8]), "+r"(r[c][9]), "+r"(r[c][10]), "+r"(r[c][11]), "+r"(r[c][12]), "+r"(r[c][13]), "+r"(r[c][14]), "+r"(r[c][15])
+                     :
+                     : "memory");
+#pragma unroll
+    for (int c = 0; c < COUNT; ++c)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[c][i] = __uint_as_float(r[c][i]);
 }
 
 // ---- matrix instruction -------------------------------------------------------------------------------------------------

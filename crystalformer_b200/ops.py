@@ -674,3 +674,55 @@ def qk_norm_bwd(q, k, wq, wk, pos, waves, eps: float, interleaved: bool, gq_out,
     ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     _call_on(dev, "cf_qk_norm_bwd", byref(args), gq_out.data_ptr(), gk_out.data_ptr(), gq.data_ptr(), gk.data_ptr(), ptr(gwq), ptr(gwk), ptr(work))
     return gq, gk, gwq, gwk
+
+
+GATE_CODES = {"silu": 0, "gelu": 1, "relu": 2}  # CF_GATE_SILU, CF_GATE_GELU, CF_GATE_RELU
+
+
+def _gated_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation: str):
+    """The description of a call, and the tensors that it points into."""
+    x = _first(x, "x", 2)
+    if activation not in GATE_CODES:
+        raise ValueError(f"activation {activation!r} is none of {', '.join(GATE_CODES)}")
+    N, D = x.shape
+    if w_gate.dim() != 2:
+        raise ValueError(f"w_gate must have 2 dimensions, got the shape {tuple(w_gate.shape)}")
+    F = w_gate.shape[0]
+    for t, name, shape in ((w_gate, "w_gate", (F, D)), (w_up, "w_up", (F, D)), (w_down, "w_down", (D, F)), (b_gate, "b_gate", (F,)),
+                           (b_up, "b_up", (F,)), (b_down, "b_down", (D,))):
+        _like(t, x, name, shape)
+    x = _rows(x)
+    rest = [None if t is None else t if t.is_contiguous() else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
+    return _lib.GatedFFN(TYPE_CODES[x.dtype], GATE_CODES[activation], N, D, F, x.data_ptr(), x.stride(0) if N > 1 else D,
+                         *[None if t is None else t.data_ptr() for t in rest]), x, rest
+
+
+def _gated_work(args, gy, device, backward: bool):
+    lib, at = _lib.load(), 0 if gy is None else gy.data_ptr()
+    if torch.cuda.current_device() == device.index:
+        nbytes = lib.cf_gated_ffn_workspace_bytes(byref(args), at, int(backward))
+    else:
+        with torch.cuda.device(device):
+            nbytes = lib.cf_gated_ffn_workspace_bytes(byref(args), at, int(backward))
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+
+
+def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation: str = "silu"):
+    """The gated feed-forward block of x (N,D): see ``feedforward.gated_feed_forward`` (cf_gated_ffn_fwd)."""
+    args, x, keep = _gated_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    work = _gated_work(args, None, x.device, False)
+    _call_on(x.device, "cf_gated_ffn_fwd", byref(args), y.data_ptr(), work.data_ptr())
+    return y
+
+
+def gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation: str, gy, wanted=(True,) * 7):
+    """Gradients of ``gated_ffn_fwd``'s seven tensors from that of its output; None where absent or not ``wanted``."""
+    args, x, keep = _gated_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
+    _like(gy, x, "gy", x.shape)
+    gy = gy.contiguous()
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None for t, want in zip((x, *keep), wanted)]
+    work = _gated_work(args, gy, x.device, True)
+    to = _lib.GatedFFNGrads(gy.data_ptr(), *[None if t is None else t.data_ptr() for t in grads])
+    _call_on(x.device, "cf_gated_ffn_bwd", byref(args), byref(to), work.data_ptr())
+    return tuple(grads)

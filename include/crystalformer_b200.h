@@ -708,6 +708,31 @@ int64_t cf_qk_norm_bwd_workspace_bytes(const cf_qk_norm *args);
 int cf_qk_norm_bwd(const cf_qk_norm *args, const void *gq_out, const void *gk_out, void *gq, void *gk, void *gwq, void *gwk,
                    void *workspace, void *stream);
 
+/* Gated feed-forward block: y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd.  x (N,D) with row stride ldx; w_gate, w_up (F,D)
+ * and w_down (D,F) contiguous; biases (F), (F), (D) or NULL; y (N,D) contiguous.  Any sizes and alignments of values; rows on 16
+ * bytes of a 16-bit type are read where they lie, others and float32 are copied into the workspace first.
+ * Backward from the same arguments and gy (N,D) contiguous: the gradients that are not NULL (gx (N,D) contiguous, the others as
+ * their parameters); g and u are computed again.  Runs of the same bits every time.
+ * workspace: cf_gated_ffn_workspace_bytes(args, gy, backward) bytes, 256-byte aligned; it depends on the addresses too, and on the
+ * device that is current. */
+#define CF_GATE_SILU 0
+#define CF_GATE_GELU 1 /* the exact one, by erf */
+#define CF_GATE_RELU 2
+typedef struct cf_gated_ffn {
+    int32_t type, activation;
+    int64_t N, D, F;
+    const void *x;
+    int64_t ldx;
+    const void *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down;
+} cf_gated_ffn;
+typedef struct cf_gated_ffn_grads {
+    const void *gy;
+    void *x, *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down;
+} cf_gated_ffn_grads;
+int64_t cf_gated_ffn_workspace_bytes(const cf_gated_ffn *args, const void *gy, int backward);
+int cf_gated_ffn_fwd(const cf_gated_ffn *args, void *y, void *workspace, void *stream);
+int cf_gated_ffn_bwd(const cf_gated_ffn *args, const cf_gated_ffn_grads *grads, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
