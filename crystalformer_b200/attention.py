@@ -29,6 +29,7 @@ from .cuda_funcs import (FusedDotProductAttentionCUDA, RealPeriodicEncodingWithP
                          ReciPeriodicEncodingFuncCUDA)
 from .cuda_funcs.kernel_manager import KernelManager
 from .params import LatticeformerParams
+from .qk_norm import QKNorm
 
 # ---------------------------------------------------------------------------------------------------------------
 # Per-batch quantities derived from the edge list: CSR offsets and the largest crystal.  The reference rebuilds the
@@ -243,6 +244,10 @@ class CrystalformerMultiheadAttentionCUDA(Module):
         self.pe_dist_proj = Parameter(torch.empty(cond, head, self.head_dim, pe_dim, **factory_kwargs)) \
             if pe_dim > 0 else None
         self.pe_wave_proj = None
+        pairs = getattr(params, "qk_rotation", 0)
+        if pairs and not getattr(params, "qk_norm", False):
+            raise ValueError("qk_rotation needs qk_norm")
+        self.qk_norm = QKNorm(num_heads, self.kdim // num_heads, pairs, **factory_kwargs) if getattr(params, "qk_norm", False) else None
         self._scale_known = False
         self._reset_parameters()
 
@@ -340,11 +345,12 @@ class CrystalformerMultiheadAttentionCUDA(Module):
     def forward(self, query: Tensor, key: Tensor, value: Tensor, batch_q: Tensor, batch_kv: Tensor, edges: Tensor,
                 points: Tensor, dist2_min: Tensor, tvecs: Tensor,
                 kr_base: Optional[Tensor] = None, rvecs: Optional[Tensor] = None, vcell: Optional[Tensor] = None,
-                onehot: Tensor = None, need_weights: bool = True, rvlen: Optional[Tensor] = None
-                ) -> Tuple[Tensor, Optional[Tensor]]:
+                onehot: Tensor = None, need_weights: bool = True, rvlen: Optional[Tensor] = None,
+                fractional: Optional[Tensor] = None) -> Tuple[Tensor, Optional[Tensor]]:
         """Same arguments as the reference (…attention_cuda.py:950-955): ``points`` is pos_ij (E,3), ``tvecs`` the
         lattice rows (B,3,3), ``rvecs`` the reciprocal rows (needed by the adaptive cut-off).  ``rvlen`` optionally
-        passes the row norms of ``rvecs`` if the caller has them already."""
+        passes the row norms of ``rvecs`` if the caller has them already.  ``fractional`` (N,3) are the atoms' fractional
+        coordinates, which a layer with ``qk_rotation`` needs."""
         P = self.params
         H = self.num_heads
         N = query.shape[0]
@@ -374,6 +380,8 @@ class CrystalformerMultiheadAttentionCUDA(Module):
         v = v.reshape(v.shape[0], H, Dv)
 
         a = self._widths(query, q)
+        if getattr(self, "qk_norm", None) is not None:  # (the widths come from the heads as projected)
+            q, k = self.qk_norm(q, k, fractional)
 
         dist_max = P.value_pe_dist_max
         if dist_max < 0:

@@ -19,6 +19,7 @@ import ctypes
 from . import _lib, ops
 from .attention import CrystalformerMultiheadAttentionCUDA, heaviest_first, register_edge_info
 from .cuda_funcs import compile_kernels
+from .feedforward import GATES, gated_feed_forward
 from .params import LatticeformerParams
 from .training import OfThisModel
 
@@ -28,7 +29,7 @@ def _get_activation_fn(activation):
         return F.relu
     if activation == "gelu":
         return F.gelu
-    raise RuntimeError("activation should be relu/gelu, not {}".format(activation))
+    raise RuntimeError("activation should be relu/gelu, or gated swiglu/geglu/reglu, not {}".format(activation))
 
 
 def _tf32(x: Tensor) -> Tensor:
@@ -104,6 +105,7 @@ class BatchGeometry:
         self.batch, self.edges, self.row_start = prep["batch"], prep["edges"], prep["row_start"]
         self.pos_ij, self.rvecs, self.vcell, self.rvlen = prep["pos_ij"], prep["rvecs"], prep["vcell"], prep["rvlen"]
         self.sizes, self.max_atoms = sizes, int(max_atoms)
+        self._pos, self._trans, self._fractional = pos, trans, None
         self.row_order = ops.row_order(self.atom_start, trans.float(), num_atoms)
         self._kr_base = None
         register_edge_info(self.edges, self.row_start, self.max_atoms, self.row_order)
@@ -115,9 +117,23 @@ class BatchGeometry:
             self._kr_base = ops.reci_phase(self.pos_ij, self.rvecs, self.batch, self.edges)
         return self._kr_base
 
+    @property
+    def fractional(self) -> Tensor:
+        """(N,3) fractional coordinates in [0, 1), built on first use, in 64 bits up to the reduction: a position moved by lattice
+        vectors has the same ones up to the rounding of the position."""
+        if self._fractional is None:
+            pos = self._pos.detach().reshape(-1, 3)[:self.batch.shape[0]].double()
+            t1, t2, t3 = self._trans.detach().reshape(-1, 3, 3).double().unbind(1)
+            rows = torch.stack((torch.linalg.cross(t2, t3), torch.linalg.cross(t3, t1), torch.linalg.cross(t1, t2)), 1)
+            rows = rows / (t1 * rows[:, 0]).sum(1)[:, None, None]
+            f = torch.einsum("nij,nj->ni", rows[self.batch], pos)
+            self._fractional = (f - f.floor()).float()
+        return self._fractional
+
 
 class CrystalformerEncoderLayerCUDA(Module):
     __constants__ = ["norm_first"]
+    gate: Optional[str] = None  # activation of a gated feed-forward block
 
     def __init__(self, d_model: int, nhead: int, dim_feedforward: int = 2048, dropout: float = 0.1,
                  activation: Union[str, Callable[[Tensor], Tensor]] = F.relu, layer_norm_eps: float = 1e-5,
@@ -136,7 +152,15 @@ class CrystalformerEncoderLayerCUDA(Module):
         self.norm2 = LayerNorm(d_model, eps=layer_norm_eps) if not no_layer_norm else Identity()
         self.dropout1 = Dropout(dropout) if dropout > 0 else Identity()
         self.dropout2 = Dropout(dropout) if dropout > 0 else Identity()
-        self.activation = _get_activation_fn(activation) if isinstance(activation, str) else activation
+        # (not the reference's) a gated block: linear_gate beside linear1, in one operator with linear2
+        if isinstance(activation, str) and activation in GATES:
+            self.gate = GATES[activation]
+            if dropout > 0:
+                raise NotImplementedError("dropout between the projections of a gated feed-forward block is not supported")
+            self.linear_gate = Linear(d_model, dim_feedforward)
+            self.activation = None
+        else:
+            self.activation = _get_activation_fn(activation) if isinstance(activation, str) else activation
         self._reset_parameters()
 
     def _reset_parameters(self):
@@ -144,6 +168,9 @@ class CrystalformerEncoderLayerCUDA(Module):
         xavier_uniform_(self.linear2.weight)
         constant_(self.linear1.bias, 0)
         constant_(self.linear2.bias, 0)
+        if self.gate is not None:
+            xavier_uniform_(self.linear_gate.weight)
+            constant_(self.linear_gate.bias, 0)
 
     def fixup_initialization(self, num_layers):
         """T-Fixup: scale four weight matrices by 0.67 L^(-1/4) (models/indexed_latticeformer_encoder.py:818-835)."""
@@ -154,23 +181,26 @@ class CrystalformerEncoderLayerCUDA(Module):
 
     def forward(self, src: Tensor, batch: Tensor, edges: Tensor, pos_ij: Tensor = None, dist2_min: Tensor = None,
                 trans: Tensor = None, kr_base: Tensor = None, rvecs: Tensor = None, vcell: Tensor = None,
-                onehot: Tensor = None, rvlen: Tensor = None) -> Tensor:
+                onehot: Tensor = None, rvlen: Tensor = None, fractional: Tensor = None) -> Tensor:
         assert pos_ij is not None and trans is not None
         x = src
         if self.norm_first:
-            x = x + self._sa_block(self.norm1(x), batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs, vcell, onehot, rvlen)
+            x = x + self._sa_block(self.norm1(x), batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs, vcell, onehot, rvlen, fractional)
             x = x + self._ff_block(self.norm2(x))
         else:
-            x = self.norm1(x + self._sa_block(x, batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs, vcell, onehot, rvlen))
+            x = self.norm1(x + self._sa_block(x, batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs, vcell, onehot, rvlen, fractional))
             x = self.norm2(x + self._ff_block(x))
         return x
 
-    def _sa_block(self, x, batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs, vcell, onehot, rvlen):
+    def _sa_block(self, x, batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs, vcell, onehot, rvlen, fractional):
         x = self.self_attn(x, x, x, batch, batch, edges, pos_ij, dist2_min, trans, kr_base, rvecs, vcell, onehot,
-                           need_weights=False, rvlen=rvlen)[0]
+                           need_weights=False, rvlen=rvlen, fractional=fractional)[0]
         return self.dropout1(x)
 
     def _ff_block(self, x: Tensor) -> Tensor:
+        if self.gate is not None:
+            return self.dropout2(gated_feed_forward(x, self.linear_gate.weight, self.linear1.weight, self.linear2.weight, self.linear_gate.bias,
+                                                    self.linear1.bias, self.linear2.bias, self.gate))
         x = self.linear2(self.dropout(self.activation(self.linear1(x))))
         return self.dropout2(x)
 
@@ -217,7 +247,7 @@ class CrystalformerEncoderCUDA(Module):
             P = att.params
             if not (P.domain in domains and P.positive_func.startswith("elu") and P.gauss_state == "q" and P.normalize_gauss and att.fused
                     and P.value_pe_condproj == "no" and P.norm_func_mode == 0 and att.kdim == 128 and att.vdim == 128
-                    and att.in_proj_bias is not None and layer.activation is F.relu and not layer.norm_first
+                    and att.in_proj_bias is not None and getattr(att, "qk_norm", None) is None and layer.activation is F.relu and not layer.norm_first
                     and isinstance(layer.norm1, Identity)):
                 return False
             if not att._scale_known:
@@ -317,7 +347,10 @@ class CrystalformerEncoderCUDA(Module):
         output = src
         for mod in self.layers:
             kr_base = g.kr_base if mod.domain != "real" else None
-            output = mod(output, g.batch, g.edges, g.pos_ij, None, trans, kr_base, g.rvecs, g.vcell, onehot, rvlen=g.rvlen)
+            norm = getattr(mod.self_attn, "qk_norm", None)
+            fractional = g.fractional if norm is not None and norm.waves is not None else None
+            output = mod(output, g.batch, g.edges, g.pos_ij, None, trans, kr_base, g.rvecs, g.vcell, onehot, rvlen=g.rvlen,
+                         fractional=fractional)
         if self.norm is not None:
             output = self.norm(output)
         return output

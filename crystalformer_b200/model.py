@@ -15,6 +15,7 @@ import torch.nn as nn
 
 from . import _lib
 from .cuda_funcs import IrregularMeanCUDA
+from .embedding import embed_species
 from .encoder import MAX_IMAGE_FF, BatchGeometry, CrystalformerEncoderCUDA, image_pointer, pack_dense_embedding, pack_dense_weight
 from .params import DEFAULT_MODEL_PARAMS, LatticeformerParams
 from .training import DOMAINS, ModelWatch, OfThisModel, train_step
@@ -39,13 +40,19 @@ def max_pool(x, batch, sizes):
     return out.scatter_reduce(0, batch[:, None].expand_as(x), x, reduce="amax", include_self=True)
 
 
+def species_of(data) -> torch.Tensor:
+    """The one-hot rows ``data.x``; where a batch has none (or None), the positions ``data.z`` of their ones."""
+    x = getattr(data, "x", None)
+    return data.z if x is None else x
+
+
 def check_batch(data, atoms: int) -> None:
     """Raises unless the tensors of ``data`` lie on one device and hold ``atoms`` atoms and the crystals of ``sizes``: the
     library gets their addresses and cannot see how long they are."""
-    x, pos, trans, sizes = data.x, data.pos, data.trans_vec, data.sizes
+    x, pos, trans, sizes = species_of(data), data.pos, data.trans_vec, data.sizes
     if x.device != pos.device or trans.device != pos.device:
         raise RuntimeError(f"x, pos and trans_vec must be on one device, not on {x.device}, {pos.device} and {trans.device}")
-    if x.dim() != 2 or sizes.dim() != 1 or x.shape[0] < atoms or pos.numel() < 3 * atoms or trans.numel() < 9 * sizes.shape[0]:
+    if x.dim() != (2 if x.is_floating_point() else 1) or sizes.dim() != 1 or x.shape[0] < atoms or pos.numel() < 3 * atoms or trans.numel() < 9 * sizes.shape[0]:
         raise ValueError(f"x {tuple(x.shape)}, pos {tuple(pos.shape)}, trans_vec {tuple(trans.shape)} and sizes {tuple(sizes.shape)} do not "
                          f"hold a batch of {atoms} atoms")
 
@@ -304,16 +311,20 @@ class Latticeformer(nn.Module):
     def forward(self, data, geometry: Optional[BatchGeometry] = None, counts: Optional[Tuple[int, int, int]] = None,
                 gather=None, inputs_ready: Optional[torch.cuda.Event] = None):
         """``data`` carries x (N,98), pos (N,3), batch (N), trans_vec (B,3,3), sizes (B) like the reference's PyG batch.
+        Without x, or with x None, z (N) whole numbers gives the position of the 1 in every row: the embedding is then a lookup
+        (``embedding.embed_species``; a position outside the row stands for padding, an embedding of zeros), the encoder as before.
         ``counts`` = (atoms, edges = sum n^2, largest crystal), when the caller knows them on the host, saves the
         device->host read of ``sizes`` (which inference overlaps with the first dense block).  ``gather`` (a ``sharding.PeerGather``, inference only): the outputs of every
         rank's crystals are returned, in the order of the unsharded batch.  ``inputs_ready`` (inference through the
         one-call path only): a CUDA event after which the tensors of ``data`` are valid.  The batch preparation, which
         depends on the inputs alone, is then not ordered behind the work already queued on the current stream and
         overlaps the previous batch's forward; the tensors must stay unchanged until this forward has run."""
-        if geometry is None and not self.training and not torch.is_grad_enabled() and data.pos.is_cuda \
+        species = species_of(data)
+        onehot = species is getattr(data, "x", None)
+        if onehot and geometry is None and not self.training and not torch.is_grad_enabled() and data.pos.is_cuda \
                 and self._native_ok():
             return self._forward_native(data, counts, gather, inputs_ready=inputs_ready)
-        if geometry is None and torch.is_grad_enabled() and data.pos.is_cuda and self._native_shell() \
+        if onehot and geometry is None and torch.is_grad_enabled() and data.pos.is_cuda and self._native_shell() \
                 and self.encoder._native_model(DOMAINS):
             y = train_step(self, data, counts)
             if y is not None:
@@ -321,7 +332,7 @@ class Latticeformer(nn.Module):
                     gather.store(y)
                     return gather.collect()
                 return y
-        x = self.input_embeddings(data.x)
+        x = self.input_embeddings(species) if onehot else embed_species(species, self.input_embeddings.weight.t())
         if geometry is None:
             geometry = BatchGeometry(data.pos, data.trans_vec, data.sizes, *(counts if counts is not None else ()))
         g = geometry

@@ -30,7 +30,9 @@ class LatticeformerParams:
                  value_pe_dist_max: float = -10.0,
                  value_pe_width_scale: float = 1.0,
                  gauss_state: str = "q",
-                 use_low_memory: bool = False) -> None:
+                 use_low_memory: bool = False,
+                 qk_norm: bool = False,
+                 qk_rotation: int = 0) -> None:
         self.layer_index = layer_index
         self.domain = domain
         self.lattice_range = lattice_range
@@ -54,6 +56,9 @@ class LatticeformerParams:
         self.value_pe_width_scale = value_pe_width_scale
         self.gauss_state = gauss_state
         self.use_low_memory = use_low_memory
+        # (not the reference's) norms of the query and key heads, and pairs of a head's entries that the positions turn
+        self.qk_norm = qk_norm
+        self.qk_rotation = qk_rotation
 
     def parseFromArgs(self, args) -> None:
         """Copies every attribute that `args` also carries (models/latticeformer_params.py:62-66)."""

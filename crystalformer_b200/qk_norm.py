@@ -66,9 +66,12 @@ class QKNorm(Module):
         self.eps = eps
         self.q_weight = Parameter(torch.ones((heads, head_dim), device=device, dtype=dtype))
         self.k_weight = Parameter(torch.ones((heads, head_dim), device=device, dtype=dtype))
-        self.register_buffer("waves", shortest_waves(heads, pairs) if pairs > 0 else None)
+        self.register_buffer("waves", shortest_waves(heads, pairs).to(device=device) if pairs > 0 else None)
 
     def forward(self, q: Tensor, k: Tensor, pos: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
         if self.waves is not None and pos is None:
             raise ValueError("the rotation needs positions")
-        return normalize_rotate(q, k, self.q_weight, self.k_weight, pos if self.waves is not None else None, self.waves, self.eps)
+        if self.waves is None:
+            return normalize_rotate(q, k, self.q_weight, self.k_weight, eps=self.eps)
+        # (a module that was converted holds its waves in 16 bits: small whole numbers, the same ones)
+        return normalize_rotate(q, k, self.q_weight, self.k_weight, pos, self.waves.float(), self.eps)

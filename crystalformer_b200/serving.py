@@ -82,13 +82,16 @@ class PipelinedPredictor:
     def _device_inputs(self, slot: int, batch):
         """Device tensors of the slot with the batch's shapes (allocated once per shape, not per batch)."""
         bufs = self._in_ring[slot]
-        shapes = (tuple(batch.x.shape), tuple(batch.pos.shape), tuple(batch.trans_vec.shape), tuple(batch.sizes.shape))
+        name = "z" if getattr(batch, "x", None) is None else "x"
+        species = getattr(batch, name)
+        shapes = (name, species.dtype, tuple(species.shape), tuple(batch.pos.shape), tuple(batch.trans_vec.shape), tuple(batch.sizes.shape))
         if bufs is None or bufs[0] != shapes:
             dev = self.device
             ns = types.SimpleNamespace(
-                x=torch.empty(shapes[0], dtype=batch.x.dtype, device=dev), pos=torch.empty(shapes[1], dtype=batch.pos.dtype, device=dev),
-                trans_vec=torch.empty(shapes[2], dtype=batch.trans_vec.dtype, device=dev),
-                sizes=torch.empty(shapes[3], dtype=torch.int64, device=dev))
+                **{name: torch.empty(species.shape, dtype=species.dtype, device=dev)},
+                pos=torch.empty(batch.pos.shape, dtype=batch.pos.dtype, device=dev),
+                trans_vec=torch.empty(batch.trans_vec.shape, dtype=batch.trans_vec.dtype, device=dev),
+                sizes=torch.empty(batch.sizes.shape, dtype=torch.int64, device=dev))
             bufs = self._in_ring[slot] = (shapes, ns)
         return bufs[1]
 
@@ -152,7 +155,7 @@ class PipelinedPredictor:
     def submit(self, batch) -> int:
         """Queues one host batch (attributes x (N,98), pos (N,3), trans_vec (B,3,3), sizes (B) int64); returns a ticket.
         Instead of the one-hot species rows ``x`` a batch may carry ``z`` (N) int64, the position of the 1 in every row
-        (only on the one-call path: 8 bytes per atom go to the device instead of 392; same outputs)."""
+        (on the one-call path, and by models that it does not take: 8 bytes per atom go to the device instead of 392; same outputs)."""
         if len(self._inflight) >= self.depth:
             raise RuntimeError("the pipeline is full: collect a result before submitting more")
         sizes_np = batch.sizes.numpy()  # host memory: no device synchronisation
@@ -185,14 +188,15 @@ class PipelinedPredictor:
                 self._inflight.append((ticket, st["events"][2], t["y_all_host"], t["status_host"]))
             self._next += 1
             return ticket
-        if getattr(batch, "x", None) is None:
-            raise ValueError("species indices `z` are taken by the one-call path only (an inference model with packed "
-                             "weights, host tensors, no `post`): pass the one-hot rows `x`")
+        if getattr(batch, "x", None) is None and self._plan is not None:
+            raise ValueError("species indices `z` are taken from host tensors, without `post`, by a model with packed weights: "
+                             "pass the one-hot rows `x`")
         dev = self._device_inputs(slot, batch)
         with torch.cuda.stream(self.copy_stream):
             if self._in_free[slot] is not None:
                 self.copy_stream.wait_event(self._in_free[slot])  # the forward that last read these buffers has run
-            dev.x.copy_(batch.x, non_blocking=True)
+            name = "x" if hasattr(dev, "x") else "z"
+            getattr(dev, name).copy_(getattr(batch, name), non_blocking=True)
             dev.pos.copy_(batch.pos, non_blocking=True)
             dev.trans_vec.copy_(batch.trans_vec, non_blocking=True)
             dev.sizes.copy_(batch.sizes, non_blocking=True)

@@ -232,6 +232,14 @@ def test_repeated_captured_and_on_a_stream():
     assert all(torch.equal(a, b) for a, b in zip(expected, captured))
 
 
+def test_module_of_another_type():
+    """Made on the device or moved there, made in a type or converted to it: the same module."""
+    from crystalformer_b200.qk_norm import QKNorm
+    q, k, _, _, pos, *_ = make(30, 4, 4, 16, 8, 3, 4, "none", torch.bfloat16, 5)
+    outs = [m(q, k, pos) for m in (QKNorm(4, 16, 8, device="cuda", dtype=torch.bfloat16), QKNorm(4, 16, 8).cuda().bfloat16())]
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and outs[0][0].dtype == torch.bfloat16
+
+
 def test_refusals():
     from crystalformer_b200 import _lib
     from crystalformer_b200.qk_norm import QKNorm, normalize_rotate
