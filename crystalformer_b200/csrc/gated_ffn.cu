@@ -28,8 +28,9 @@ struct PackJob {
     int cols;
     Planes to;
     long long groups;  // of eight values, with those that pad a row
+    bool transposed;   // rows and cols are those of the planes, the source's the other way round
 };
-constexpr int PACK_JOBS = 5;
+constexpr int PACK_JOBS = 5, COLUMN_SHARES = 256;
 struct PackJobs {
     PackJob j[PACK_JOBS];
 };
@@ -45,24 +46,27 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
     const T *src = static_cast<const T *>(job.src);
     P *to = static_cast<P *>(job.to.base);
     const bool wide = ((reinterpret_cast<uintptr_t>(src) & 15) | (job.ld % (16 / (int)sizeof(T)))) == 0;
-    const int per_row = (int)(job.to.ld / 8);
+    const long long per_row = job.to.ld / 8;
     for (long long g = (long long)blockIdx.x * 256 + threadIdx.x; g < job.groups; g += (long long)gridDim.x * 256) {
-        const long long row = g / per_row;
-        const int col = (int)(g - row * per_row) * 8, room = job.cols - col;
-        const T *at = src + row * job.ld + col;
+        // (neighbouring threads read neighbours: along the source's rows)
+        const long long row = job.transposed ? g % job.rows : g / per_row;
+        const int col = (int)(job.transposed ? g / job.rows : g - row * per_row) * 8, room = job.cols - col;
         float v[8];
-        if (wide && room >= 8) {
+        if (job.transposed) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < room ? to_float(src[(col + i) * job.ld + row]) : 0.f;
+        } else if (wide && room >= 8) {
             constexpr int VEC = 16 / sizeof(T);
 #pragma unroll
             for (int i = 0; i < 8; i += VEC) {
                 float w[VEC];
-                load_values<T, VEC>(at + i, w);
+                load_values<T, VEC>(src + row * job.ld + col + i, w);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[i + e] = w[e];
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = i < room ? to_float(at[i]) : 0.f;
+            for (int i = 0; i < 8; ++i) v[i] = i < room ? to_float(src[row * job.ld + col + i]) : 0.f;
         }
         uint32_t w[NP][4];
 #pragma unroll
@@ -112,42 +116,62 @@ __global__ void __launch_bounds__(256) share_sum_kernel(const ShareArgs p)
     }
 }
 
-// ---- sums of columns (the biases' gradients): blocks of 64 columns x a share of the rows, then the shares in their order -----------
-constexpr int COLUMN_SHARES = 64;
-template <class P, int NP>
-__global__ void __launch_bounds__(256) column_share_kernel(const P *x, long long ld, long long plane, long long rows, int cols, float *partial)
+// ---- sums of columns (the biases' gradients) --------------------------------------------------------------------------------------
+// Shares of the rows of a matrix: a block's eight warps take rows in turn, a lane VEC columns, and add up at the end.
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) column_share_kernel(const T *x, long long rows, int cols, float *partial)
 {
-    __shared__ float part[4][64];
+    __shared__ float part[8][32 * VEC];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, col = blockIdx.x * 64 + c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = (blockIdx.x * 32 + lane) * VEC;
     const long long lo = rows * blockIdx.y / gridDim.y, hi = rows * (blockIdx.y + 1) / gridDim.y;
-    float sum = 0.f, low = 0.f;
+    float sum[VEC], low[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum[e] = low[e] = 0.f;
     if (col < cols) {
 #pragma unroll 4
-        for (long long n = lo + r; n < hi; n += 4) {
-            float v = to_float(x[n * ld + col]);
-            if constexpr (NP == 3) v += to_float(x[plane + n * ld + col]) + to_float(x[2 * plane + n * ld + col]);
-            add_compensated(v, sum, low);
+        for (long long n = lo + warp; n < hi; n += 8) {
+            float v[VEC];
+            load_values<T, VEC>(x + n * cols + col, v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) add_compensated(v[e], sum[e], low[e]);
         }
     }
-    part[r][c] = sum + low;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) part[warp][e * 32 + lane] = sum[e] + low[e];
     __syncthreads();
-    if (r == 0 && col < cols) partial[(long long)blockIdx.y * cols + col] = (part[0][c] + part[1][c]) + (part[2][c] + part[3][c]);
+    for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+        const int at = (blockIdx.x * 32 + (i & 31)) * VEC + (i >> 5);
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += part[w][i];
+        if (at < cols) partial[(long long)blockIdx.y * cols + at] = t;
+    }
 }
+// Shares added: to fewer of them (`fewer`, gridDim.y of them), or to the columns' places in the gradients.
 template <class T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float *partial, int shares, int cols, T *out0, int cols0, T *out1, int col1, int cols1)
+__global__ void __launch_bounds__(256) column_sum_kernel(const float *partial, long long shares, int cols, float *fewer, T *out0, int cols0, T *out1, int col1,
+                                                         int cols1)
 {
+    __shared__ float part[8][32];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int col = blockIdx.x * 256 + threadIdx.x;
-    if (col >= cols) return;
-    T *to = col < cols0 ? (out0 ? out0 + col : nullptr) : col >= col1 && col < col1 + cols1 && out1 ? out1 + (col - col1) : nullptr;
-    if (to == nullptr) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
+    const long long lo = shares * blockIdx.y / gridDim.y, hi = shares * (blockIdx.y + 1) / gridDim.y;
     float t = 0.f;
+    if (col < cols) {
 #pragma unroll 8
-    for (int s = 0; s < shares; ++s) t += partial[(long long)s * cols + col];
-    *to = from_float<T>(t);
+        for (long long s = lo + warp; s < hi; s += 8) t += partial[s * cols + col];
+    }
+    part[warp][lane] = t;
+    __syncthreads();
+    if (warp > 0 || col >= cols) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) t += part[w][lane];
+    if (fewer != nullptr) fewer[(long long)blockIdx.y * cols + col] = t;
+    else if (col < cols0) { if (out0 != nullptr) out0[col] = from_float<T>(t); }
+    else if (col >= col1 && col < col1 + cols1) { if (out1 != nullptr) out1[col - col1] = from_float<T>(t); }
 }
 
 // ---- tensor maps ----------------------------------------------------------------------------------------------------------------------
@@ -191,23 +215,42 @@ struct Operand {
 };
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------------
-template <class T, int MODE, int TN>
+template <class T, int MODE, int TN, bool PAIR>
 int launch_tiles(const Params &p, bool chained, cudaStream_t s)
 {
-    using S = Shape<T, MODE, TN>;
-    static thread_local bool configured[64] = {};
+    using S = Shape<T, MODE, TN, PAIR>;
+    static thread_local int resident[64] = {};  // blocks that the GPU holds at a time (0: not asked yet)
     int dev = 0;
     cudaGetDevice(&dev);
-    if (!configured[dev & 63]) {
-        if (cudaFuncSetAttribute(tile_kernel<T, MODE, TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
+    int &blocks = resident[dev & 63];
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PAIR ? 2 : 1; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (blocks == 0) {
+        if (cudaFuncSetAttribute(tile_kernel<T, MODE, TN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) {
             cudaGetLastError();
             return fail(CF_ERR_CUDA, "cf_gated_ffn: %d bytes of shared memory not available", S::SMEM);
         }
-        configured[dev & 63] = true;
+        int clusters = 0;
+        cfg.gridDim = dim3(2 * (unsigned)sm_count());
+        if (PAIR && (cudaOccupancyMaxActiveClusters(&clusters, tile_kernel<T, MODE, TN, PAIR>, &cfg) != cudaSuccess || clusters < 1)) {
+            cudaGetLastError();
+            clusters = sm_count() / 2;
+        }
+        blocks = PAIR ? std::min(2 * clusters, sm_count()) : sm_count();
     }
-    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits, cap = sm_count();
-    if (launch_chained(tile_kernel<T, MODE, TN>, dim3((unsigned)std::min(tiles, cap)), dim3(THREADS), S::SMEM, s, chained, p) != cudaSuccess)
-        return launch_status("tile_kernel");
+    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
+    cfg.gridDim = dim3((unsigned)std::min<long long>(PAIR ? 2 * tiles : tiles, blocks));
+    cfg.numAttrs = chained && chained_launches_enabled() ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, tile_kernel<T, MODE, TN, PAIR>, p) != cudaSuccess) return launch_status("tile_kernel");
     return launch_status("tile_kernel");
 }
 
@@ -229,27 +272,34 @@ struct Linear {
 
 int blocks_of(long long K) { return (int)((K + TK - 1) / TK); }
 
-// Width of the tiles and number of shares: the cheapest of the kernel's waves (blocks of the contraction, and what a tile costs beside
-// them) and of the shares' way through memory, in units of a block of a 128-wide tile.
+// Width of the tiles, one block or a pair of them to a tile, and number of shares: the cheapest of the kernel's rounds (blocks of the
+// contraction, and what a tile costs beside them) and of the shares' way through memory.  Unit: 256 clocks, the products of
+// 128 x 128 x 64 values of 16 bits.
 struct Cut {
-    int tn, splits;
+    int tn;
+    bool pair;
+    int splits;
 };
 template <class T>
 Cut linear_cut(long long M, int N, int blocks)
 {
+    // a block of the contraction of a 16-bit type: its products, or (tiles of one block) what L2 delivers; of float32: six products
+    struct Kind { int tn; bool pair; double one, six; };
+    constexpr Kind kinds[] = {{256, true, 2.0, 12.5}, {128, true, 1.15, 6.6}, {128, false, 1.7, 7.2}, {64, false, 1.2, 4.4}};
+    constexpr bool wide = pieces_of<T> > 1;
     const double sms = sm_count();
-    Cut best{128, 1};
+    Cut best{128, false, 1};
     double least = 1e300;
-    for (int tn : {128, 64}) {
-        const double tiles = (double)((M + TM - 1) / TM) * ((N + tn - 1) / tn);
+    for (const Kind &k : kinds) {
+        const double tiles = (double)((M + (k.pair ? 255 : 127)) / (k.pair ? 256 : 128)) * ((N + k.tn - 1) / k.tn);
         for (int sp = 1; sp <= 64 && sp <= blocks; sp = sp < 4 ? sp + 1 : sp + sp / 4) {
-            const double waves = std::ceil(tiles * sp / sms), block = tn == 128 ? 1.0 : 0.7;
-            // a tile's set-up and epilogue: about six blocks of its products; shares: 8 bytes a value, a launch
-            const double cost = waves * (std::ceil((double)blocks / sp) * block + (pieces_of<T> > 1 ? 1.5 : 6.0)) +
-                                (sp > 1 ? (pieces_of<T> > 1 ? 4.0 : 12.0) + (double)sp * M * N * (pieces_of<T> > 1 ? 2e-6 : 6e-6) : 0.0);
+            const double rounds = std::ceil(tiles * sp / (k.pair ? std::floor(sms / 2) : sms));
+            // a tile's start and the last one's epilogue: some 8 units; shares: a launch, and 8 bytes a value at 13 KB a unit
+            const double cost = rounds * std::ceil((double)blocks / sp) * (wide ? k.six : k.one) + 8.0 + 3.0 * rounds +
+                                (sp > 1 ? 16.0 + (double)sp * M * N * 8.0 / 1e6 : 0.0);
             if (cost < least * 0.99) {
                 least = cost;
-                best = {tn, sp};
+                best = {k.tn, k.pair, sp};
             }
         }
     }
@@ -274,12 +324,13 @@ int run_linear(const Linear &l, float *partial, cudaStream_t s)
         p.a_across[i] = l.a_across[i];
         p.b_across[i] = l.b_across[i];
         int rc = encode<T>(&p.a[i], l.a[i].x, l.a[i].rows, l.a[i].cols, l.a_across[i] ? TK : TM);
-        if (rc == CF_OK) rc = encode<T>(&p.b[i], l.b[i].x, l.b[i].rows, l.b[i].cols, l.b_across[i] ? TK : cut.tn);
+        if (rc == CF_OK) rc = encode<T>(&p.b[i], l.b[i].x, l.b[i].rows, l.b[i].cols, l.b_across[i] ? TK : cut.pair ? cut.tn / 2 : cut.tn);
         if (rc != CF_OK) return rc;
     }
     p.M = l.M;
     p.N = l.N;
-    p.m_tiles = (int)((l.M + TM - 1) / TM);
+    const int tm = cut.pair ? 2 * TM : TM;
+    p.m_tiles = (int)((l.M + tm - 1) / tm);
     p.n_tiles = (l.N + cut.tn - 1) / cut.tn;
     p.splits = cut.splits;
     p.out0 = l.out0; p.out1 = l.out1;
@@ -287,7 +338,8 @@ int run_linear(const Linear &l, float *partial, cudaStream_t s)
     p.bias = l.bias;
     p.partial = cut.splits > 1 ? partial : nullptr;
     p.status = wait_status();
-    const int rc = cut.tn == 128 ? launch_tiles<T, LINEAR, 128>(p, true, s) : launch_tiles<T, LINEAR, 64>(p, true, s);
+    const int rc = cut.tn == 256 ? launch_tiles<T, LINEAR, 256, true>(p, true, s) : cut.pair ? launch_tiles<T, LINEAR, 128, true>(p, true, s) :
+                   cut.tn == 128 ? launch_tiles<T, LINEAR, 128, false>(p, true, s) : launch_tiles<T, LINEAR, 64, false>(p, true, s);
     if (rc != CF_OK || cut.splits == 1) return rc;
     const ShareArgs sum{partial, cut.splits, l.N, l.M, l.out0, l.out1, l.rows0, l.row1, l.rows1, l.ld_out, l.bias};
     if (launch_chained(share_sum_kernel<T>, dim3(stride_blocks(l.M * l.N)), dim3(256), 0, s, true, sum) != cudaSuccess) return launch_status("share_sum_kernel");
@@ -295,7 +347,7 @@ int run_linear(const Linear &l, float *partial, cudaStream_t s)
 }
 
 // ---- plans: where the operands of a call lie ------------------------------------------------------------------------------------------------
-long long round8(long long n) { return (n + 7) & ~7ll; }
+long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
 
 template <class T>
 struct Plan {
@@ -304,28 +356,29 @@ struct Plan {
     const cf_gated_ffn &d;
     long long Fp;
     Operand x, wg, wu, wd, gy, h, dg, du;
-    float *partial;
+    float *partial, *sums = nullptr;  // sums: of the columns of dg and du, 32 rows each
     size_t bytes;
     PackJobs jobs{};
     int job_count = 0;
 
     // The matrix itself where TMA can read it (16-bit types on 16 bytes), else its planes in the workspace and the job that makes them.
-    Operand place(Carver &c, const void *src, long long rows, long long cols, long long ld)
+    Operand place(Carver &c, const void *src, long long rows, long long cols, long long ld, bool transposed = false)
     {
-        if (NP == 1 && aligned_to(src, 16) && ld % 8 == 0 && ld >= cols && ld < (1ll << 38)) return {{const_cast<void *>(src), ld, 0}, rows, cols};
-        const long long to_ld = round8(cols), plane = rows * to_ld;
+        if (NP == 1 && !transposed && aligned_to(src, 16) && ld % 8 == 0 && ld >= cols && ld < (1ll << 38)) return {{const_cast<void *>(src), ld, 0}, rows, cols};
+        const long long to_ld = round_up(cols, 8), plane = rows * to_ld;
         P *to = c.take<P>((size_t)NP * plane);
-        jobs.j[job_count++] = {src, rows, ld, (int)cols, {to, to_ld, plane}, rows * (to_ld / 8)};
+        jobs.j[job_count++] = {src, rows, ld, (int)cols, {to, to_ld, plane}, rows * (to_ld / 8), transposed};
         return {{to, to_ld, plane}, rows, cols};
     }
 
-    Plan(const cf_gated_ffn &args, const void *gy_src, bool backward, void *base) : d(args), Fp(round8(args.F))
+    Plan(const cf_gated_ffn &args, const void *gy_src, bool backward, void *base) : d(args), Fp(round_up(args.F, 16))
     {
         Carver c{static_cast<char *>(base)};
         x = place(c, d.x, d.N, d.D, d.ldx);
         wg = place(c, d.w_gate, d.F, d.D, d.D);
         wu = place(c, d.w_up, d.F, d.D, d.D);
-        wd = place(c, d.w_down, d.D, d.F, d.F);
+        // (the backward's product with it runs across its rows; three pieces, which are packed anyway, are packed transposed)
+        wd = backward && NP == 3 ? place(c, d.w_down, d.F, d.D, d.F, true) : place(c, d.w_down, d.D, d.F, d.F);
         if (backward) gy = place(c, gy_src, d.N, d.D, d.D);
         P *hm = c.take<P>((size_t)NP * d.N * Fp);
         h = {{hm, Fp, d.N * Fp}, d.N, d.F};
@@ -339,6 +392,7 @@ struct Plan {
             const int rows = blocks_of(d.N);
             floats = std::max<size_t>({linear_partial<T>(d.N, (int)d.D, 2 * blocks_of(d.F)), linear_partial<T>(2 * Fp, (int)d.D, rows),
                                linear_partial<T>(d.D, (int)d.F, rows), (size_t)(COLUMN_SHARES * std::max<long long>(2 * Fp, d.D))});
+            sums = c.take<float>((size_t)((d.N + 31) / 32) * 2 * Fp);
         }
         partial = c.take<float>(floats);
         bytes = c.used;
@@ -356,27 +410,35 @@ int run_pack(const Plan<T> &plan, cudaStream_t s)
 }
 
 template <class T>
-int run_glu(const Plan<T> &plan, bool backward, cudaStream_t s)
+int run_glu(const Plan<T> &plan, bool backward, bool sums, cudaStream_t s)
 {
     const cf_gated_ffn &d = plan.d;
+    constexpr bool wide = pieces_of<T> > 1;
     Params p{};
-    const long long m_tiles = (d.N + TM - 1) / TM;
-    // three pieces leave shared memory for two stages of 64-wide tiles; one piece takes the wide tiles unless they leave SMs idle
-    const int tn = pieces_of<T> > 1 || m_tiles * ((d.F + 127) / 128) < sm_count() ? 64 : 128;
+    // Tiles of pairs (256 x 128; backward in three pieces, whose sums must fit registers, 256 x 64) or of single blocks (128 x 64): the
+    // cheaper by rounds times products, single blocks' bound by L2 (16 bits).
+    const int pair_tn = wide && backward ? 64 : 128;
+    const double sms = sm_count();
+    auto rounds = [&](int tm, int tn, double at_once) { return std::ceil((double)((d.N + tm - 1) / tm) * ((d.F + tn - 1) / tn) / at_once); };
+    const double blocks = blocks_of(d.D);
+    const bool pair = rounds(256, pair_tn, std::floor(sms / 2)) * pair_tn * (blocks + 2) < rounds(128, 64, sms) * 64 * (blocks + 2) * (wide ? 1.1 : 1.4);
+    const int tn = pair ? pair_tn : 64, tm = pair ? 2 * TM : TM;
+    const int of_x = backward ? 1 : 0;
     p.blocks0 = blocks_of(d.D);
     p.blocks = backward ? 2 * p.blocks0 : p.blocks0;
-    int rc = encode<T>(&p.a[0], plan.x.x, d.N, d.D, TM);
-    if (rc == CF_OK) rc = encode<T>(&p.b[0], plan.wg.x, d.F, d.D, tn);
-    if (rc == CF_OK) rc = encode<T>(&p.b[1], plan.wu.x, d.F, d.D, tn);
+    int rc = encode<T>(&p.a[of_x], plan.x.x, d.N, d.D, TM);
+    if (rc == CF_OK) rc = encode<T>(&p.b[1], plan.wg.x, d.F, d.D, tn);
+    if (rc == CF_OK) rc = encode<T>(&p.b[2], plan.wu.x, d.F, d.D, tn);
     if (backward) {
-        if (rc == CF_OK) rc = encode<T>(&p.a[1], plan.gy.x, d.N, d.D, TM);
-        if (rc == CF_OK) rc = encode<T>(&p.b[2], plan.wd.x, d.D, d.F, TK);
-        p.b_across[1] = 1;
+        if (rc == CF_OK) rc = encode<T>(&p.a[0], plan.gy.x, d.N, d.D, TM);
+        if (rc == CF_OK) rc = wide ? encode<T>(&p.b[0], plan.wd.x, d.F, d.D, pair ? tn / 2 : tn) : encode<T>(&p.b[0], plan.wd.x, d.D, d.F, TK);
+        p.b_across[0] = !wide;
         p.dg = plan.dg.x;
         p.du = plan.du.x;
+        p.sums = sums ? plan.sums : nullptr;
     }
     if (rc != CF_OK) return rc;
-    p.m_tiles = (int)m_tiles;
+    p.m_tiles = (int)((d.N + tm - 1) / tm);
     p.n_tiles = (int)((d.F + tn - 1) / tn);
     p.splits = 1;
     p.M = d.N;
@@ -388,10 +450,8 @@ int run_glu(const Plan<T> &plan, bool backward, cudaStream_t s)
     p.padded = (int)plan.Fp;
     p.status = wait_status();
     const bool chained = plan.job_count > 0;
-    if constexpr (pieces_of<T> == 1) {
-        if (tn == 128) return backward ? launch_tiles<T, GLU_BACKWARD, 128>(p, chained, s) : launch_tiles<T, GLU_FORWARD, 128>(p, chained, s);
-    }
-    return backward ? launch_tiles<T, GLU_BACKWARD, 64>(p, chained, s) : launch_tiles<T, GLU_FORWARD, 64>(p, chained, s);
+    if (!pair) return backward ? launch_tiles<T, GLU_BACKWARD, 64, false>(p, chained, s) : launch_tiles<T, GLU_FORWARD, 64, false>(p, chained, s);
+    return backward ? launch_tiles<T, GLU_BACKWARD, wide ? 64 : 128, true>(p, chained, s) : launch_tiles<T, GLU_FORWARD, 128, true>(p, chained, s);
 }
 
 template <class T>
@@ -400,7 +460,7 @@ int forward(const cf_gated_ffn &d, void *y, void *workspace, cudaStream_t s)
     if (d.N <= GATED_ROWS) return gated_rows<T>(d, y, static_cast<float *>(workspace), s);
     const Plan<T> plan(d, nullptr, false, workspace);
     int rc = run_pack(plan, s);
-    if (rc == CF_OK) rc = run_glu(plan, false, s);
+    if (rc == CF_OK) rc = run_glu(plan, false, false, s);
     if (rc != CF_OK) return rc;
     Linear l{};
     l.a[0] = plan.h; l.b[0] = plan.wd;
@@ -412,17 +472,31 @@ int forward(const cf_gated_ffn &d, void *y, void *workspace, cudaStream_t s)
     return run_linear<T>(l, plan.partial, s);
 }
 
+// The shares of columns in `from` (through `fewer` where they are many) to their places.
 template <class T>
-int column_sums(const Planes &x, int np, long long rows, int cols, float *partial, T *out0, int cols0, T *out1, int col1, int cols1, bool typed, cudaStream_t s)
+int column_sums(const float *from, long long shares, int cols, float *fewer, T *out0, int cols0, T *out1, int col1, int cols1, cudaStream_t s)
 {
-    using P = typename Piece<T>::type;
-    const dim3 grid((cols + 63) / 64, (unsigned)std::max(1ll, std::min<long long>(COLUMN_SHARES, rows / 32)));
-    cudaError_t err;
-    if (typed) err = launch_chained(column_share_kernel<T, 1>, grid, dim3(256), 0, s, true, static_cast<const T *>(x.base), x.ld, x.plane, rows, cols, partial);
-    else err = launch_chained(column_share_kernel<P, pieces_of<T>>, grid, dim3(256), 0, s, true, static_cast<const P *>(x.base), x.ld, x.plane, rows, cols, partial);
-    if (err == cudaSuccess)
-        err = launch_chained(column_sum_kernel<T>, dim3((cols + 255) / 256), dim3(256), 0, s, true, partial, (int)grid.y, cols, out0, cols0, out1, col1, cols1);
+    const unsigned groups = (unsigned)(cols + 31) / 32;
+    if (shares > 256) {
+        const unsigned to = (unsigned)std::min<long long>(COLUMN_SHARES, shares / 64);
+        launch_chained(column_sum_kernel<T>, dim3(groups, to), dim3(256), 0, s, true, from, shares, cols, fewer, out0, cols0, out1, col1, cols1);
+        from = fewer;
+        shares = to;
+    }
+    launch_chained(column_sum_kernel<T>, dim3(groups), dim3(256), 0, s, true, from, shares, cols, static_cast<float *>(nullptr), out0, cols0, out1, col1, cols1);
     return launch_status("column_sum_kernel");
+}
+
+template <class T>
+int row_sums(const T *x, long long rows, int cols, float *partial, T *out, cudaStream_t s)
+{
+    constexpr int VEC = 16 / sizeof(T);
+    const bool wide = cols % VEC == 0 && aligned_to(x, 16);
+    const unsigned groups = (unsigned)(cols + (wide ? 32 * VEC : 32) - 1) / (wide ? 32 * VEC : 32);
+    const unsigned shares = (unsigned)std::max(1ll, std::min<long long>(COLUMN_SHARES, rows / 32));
+    if (wide) launch_chained(column_share_kernel<T, VEC>, dim3(groups, shares), dim3(256), 0, s, true, x, rows, cols, partial);
+    else launch_chained(column_share_kernel<T, 1>, dim3(groups, shares), dim3(256), 0, s, true, x, rows, cols, partial);
+    return column_sums<T>(partial, shares, cols, nullptr, out, cols, nullptr, cols, 0, s);
 }
 
 template <class T>
@@ -430,7 +504,7 @@ int backward(const cf_gated_ffn &d, const cf_gated_ffn_grads &g, void *workspace
 {
     const Plan<T> plan(d, g.gy, true, workspace);
     int rc = run_pack(plan, s);
-    if (rc == CF_OK) rc = run_glu(plan, true, s);
+    if (rc == CF_OK) rc = run_glu(plan, true, g.b_gate || g.b_up, s);
     if (rc != CF_OK) return rc;
     const int D = (int)d.D, F = (int)d.F;
     const long long Fp = plan.Fp;
@@ -468,10 +542,10 @@ int backward(const cf_gated_ffn &d, const cf_gated_ffn_grads &g, void *workspace
         if ((rc = run_linear<T>(l, plan.partial, s)) != CF_OK) return rc;
     }
     if (g.b_gate || g.b_up) {
-        rc = column_sums<T>(plan.dg.x, pieces_of<T>, d.N, (int)(2 * Fp), plan.partial, static_cast<T *>(g.b_gate), F, static_cast<T *>(g.b_up), (int)Fp, F, false, s);
+        rc = column_sums<T>(plan.sums, (d.N + 31) / 32, (int)(2 * Fp), plan.partial, static_cast<T *>(g.b_gate), F, static_cast<T *>(g.b_up), (int)Fp, F, s);
         if (rc != CF_OK) return rc;
     }
-    if (g.b_down) rc = column_sums<T>({const_cast<void *>(g.gy), D, 0}, 1, d.N, D, plan.partial, static_cast<T *>(g.b_down), D, nullptr, D, 0, true, s);
+    if (g.b_down) rc = row_sums<T>(static_cast<const T *>(g.gy), d.N, D, plan.partial, static_cast<T *>(g.b_down), s);
     return rc;
 }
 

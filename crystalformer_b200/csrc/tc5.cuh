@@ -75,6 +75,34 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void *map, int x
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
+// ... of a pair of blocks (cta_group::2): the barrier may be the other block's (`bar` from mapa)
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void *map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+// the address of a place in this block's shared memory in that of block `rank` of the cluster
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar)  // an address from mapa
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+    return r;
+}
 // ordinary shared-memory writes of this thread become visible to tcgen05.mma (the asynchronous proxy)
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -92,6 +120,18 @@ __device__ __forceinline__ void tmem_free(uint32_t addr)  // the same warp
 {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "n"(COLUMNS) : "memory");
 }
+// ... of both blocks of a pair: a warp of either
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t result_smem)
+{
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(result_smem), "n"(COLUMNS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+template <int COLUMNS>
+__device__ __forceinline__ void tmem_free_pair(uint32_t addr)
+{
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "n"(COLUMNS) : "memory");
+}
 // 16 lanes x 32 columns of 32-bit accumulators, laid out as the C fragments of four 16 x 8 tiles: register 4 j + u of
 // lane (g = lane / 4, t = lane % 4) is row g + 8 (u / 2), column 8 j + 2 t + u % 2.
 __device__ __forceinline__ void tmem_load_16x32(uint32_t addr, float (&v)[16])
@@ -108,9 +148,10 @@ __device__ __forceinline__ void tmem_load_16x32(uint32_t addr, float (&v)[16])
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// 32 lanes (the warp's quarter of the 128) x 16 columns: lane l has row l.  Of COUNT accumulators at once, `apart` columns apart.
+// 32 lanes (the warp's quarter of the 128) x 16 columns: lane l has row l.  Of COUNT accumulators at once, `apart` columns apart,
+// the third one `more` further.
 template <int COUNT>
-__device__ __forceinline__ void tmem_load_rows16(uint32_t addr, uint32_t apart, float (&v)[COUNT][16])
+__device__ __forceinline__ void tmem_load_rows16(uint32_t addr, uint32_t apart, float (&v)[COUNT][16], uint32_t more)
 {
     uint32_t r[COUNT][16];
 #pragma unroll
@@ -118,7 +159,7 @@ __device__ __forceinline__ void tmem_load_rows16(uint32_t addr, uint32_t apart, 
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                      : "=r"(r[c][0]), "=r"(r[c][1]), "=r"(r[c][2]), "=r"(r[c][3]), "=r"(r[c][4]), "=r"(r[c][5]), "=r"(r[c][6]), "=r"(r[c][7]),
                        "=r"(r[c][8]), "=r"(r[c][9]), "=r"(r[c][10]), "=r"(r[c][11]), "=r"(r[c][12]), "=r"(r[c][13]), "=r"(r[c][14]), "=r"(r[c][15])
-                     : "r"(addr + (uint32_t)c * apart)
+                     : "r"(addr + (uint32_t)c * apart + (c == 2 ? more : 0u))
                      : "memory");
     // (the registers pass through the wait, so that nothing reads them before it)
 #pragma unroll
@@ -158,6 +199,20 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint
 __device__ __forceinline__ void mma_commit(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+// ... of a pair of blocks, issued by the first: either block holds 128 rows of A, half of the rows of B and its rows of D
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+                 "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+                 : "memory");
+}
+// the barriers at the same place of both blocks
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                 : "memory");
 }
 
 // ---- two-piece operands -----------------------------------------------------------------------------------------------

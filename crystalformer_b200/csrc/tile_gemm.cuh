@@ -3,12 +3,15 @@
 //   LINEAR        C = A0 B0^T [+ A1 B1^T]                       epilogue: bias, stored in the type of the call; or float32 shares of a
 //                                                               split contraction, which a second kernel adds
 //   GLU_FORWARD   g = X Wg^T, u = X Wu^T                        epilogue: h = act(g + bg) (u + bu)
-//   GLU_BACKWARD  the same, then dh = Gy Wd                     epilogue: h, dg = dh u act'(g), du = dh act(g)
+//   GLU_BACKWARD  dh = Gy Wd, then the same                     epilogue: h, dg = dh u act'(g), du = dh act(g), sums of columns of 32 rows
 //
-// A block holds a 128 x TN tile of each accumulator in tensor memory and walks the contraction in blocks of 64: one thread keeps
-// STAGES of them in flight by TMA (128-byte swizzle; either order of an operand, its contraction running along or across its rows), one
-// thread issues tcgen05.mma, eight warps take the accumulators.  The grid is as large as the GPU and every block walks tiles, so
-// that, with two sets of accumulators, a tile's epilogue runs beside the next one's products.
+// A block holds a 128-row tile of each accumulator in tensor memory, TN columns wide, and walks the contraction in blocks of 64: one
+// thread keeps STAGES of them in flight by TMA (128-byte swizzle; either order of an operand, its contraction running along or across
+// its rows), one thread issues tcgen05.mma, sixteen warps take the accumulators.  PAIR: two blocks of a cluster share their products
+// (cta_group::2, 256 rows): each fetches half of B, which halves what a block of the contraction moves from L2 (32 KB per 128 x 256
+// products of 64; the tiles of one block are bound by that).  The grid is as large as the GPU and every block walks tiles, so that a
+// tile's epilogue runs beside the next one's products: two sets of accumulators; GLU_BACKWARD of 16-bit types, whose set is 384 of
+// the 512 columns, has two of dh alone and computes the next tile's dh beside the epilogue.
 //
 // 16-bit types: one product per pair of blocks; rows of 64 values are 128 bytes.  float32: an operand is the sum of three bfloat16
 // pieces (24 bits, any exponent), made once by a packing kernel or by the epilogue that produces it, and a product is six: piece 0
@@ -19,6 +22,8 @@
 // All waits are bounded (tc5::mbar_wait); one that runs out ends the block after its copies and products in flight.
 #pragma once
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc5.cuh"
@@ -31,7 +36,7 @@ enum Mode { LINEAR = 0, GLU_FORWARD = 1, GLU_BACKWARD = 2 };
 enum Activation { SILU = 0, GELU = 1, RELU = 2 };
 
 constexpr int TM = 128, TK = 64;
-constexpr int EPILOGUE_WARPS = 8, THREADS = (EPILOGUE_WARPS + 2) * 32;
+constexpr int EPILOGUE_WARPS = 16, THREADS = (EPILOGUE_WARPS + 2) * 32;
 
 template <class T> constexpr int pieces_of = sizeof(T) == 4 ? 3 : 1;
 template <class T> struct Piece { using type = T; };
@@ -44,17 +49,19 @@ struct Planes {
 };
 
 struct Params {
-    CUtensorMap a[2], b[3];   // LINEAR: a[0] with b[0], a[1] with b[1]; GLU: a[0] with b[0] (gate) and b[1] (up), a[1] with b[2]
+    // LINEAR: a[0] with b[0], a[1] with b[1]; GLU: x with b[1] (gate) and b[2] (up), backward: gy = a[0] with b[0] (down), x = a[1]
+    CUtensorMap a[2], b[3];
     int a_across[2], b_across[2];  // per part: the contraction runs across the rows of the operand
     int blocks0, blocks;      // of the contraction: of the first part, of both
-    int m_tiles, n_tiles, splits;
+    int m_tiles, n_tiles, splits;  // m_tiles: of 128 rows, or 256 of a pair
     long long M;
     int N;
     // GLU
     const void *bias_gate, *bias_up;
     int act;
     Planes h, dg, du;
-    int padded;               // columns that h, dg and du have memory for
+    int padded;               // columns that h, dg and du have memory for, a multiple of 16
+    float *sums;              // or null: (32 rows each, 2 padded) sums of the columns of dg and du
     // LINEAR: rows [0, rows0) to out0, rows [row1, row1 + rows1) to out1
     void *out0, *out1;
     long long rows0, row1, rows1, ld_out;
@@ -63,21 +70,24 @@ struct Params {
     unsigned *status;
 };
 
-template <class T, int MODE, int TN>
+template <class T, int MODE, int TN, bool PAIR>
 struct Shape {
     static constexpr int NP = pieces_of<T>;
-    static constexpr int NB = MODE == LINEAR ? 1 : 2;                     // tiles of B per block of the contraction
+    // rows of B that a block fetches per block of the contraction: of both projections, of a single matrix
+    static constexpr int ROWS_GU = PAIR ? TN : 2 * TN, ROWS_ONE = PAIR ? TN / 2 : TN, ROWS = MODE == LINEAR ? ROWS_ONE : ROWS_GU;
     static constexpr int ACCS = MODE == LINEAR ? 1 : MODE == GLU_FORWARD ? 2 : 3;
-    static constexpr int A_PIECE = TM * TK * 2, B_PIECE = NB * TN * TK * 2;
+    static constexpr int A_PIECE = TM * TK * 2, B_PIECE = ROWS * TK * 2;
     static constexpr int STAGE = NP * (A_PIECE + B_PIECE);
-    static constexpr int ROOM = 222 * 1024;
+    static constexpr int ROOM = 220 * 1024;
     static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
-    static constexpr int COLUMNS = ACCS * TN;                             // of one set of accumulators
-    static constexpr int SETS = 2 * COLUMNS <= 512 ? 2 : 1;
-    static constexpr int TMEM = SETS * COLUMNS <= 64 ? 64 : SETS * COLUMNS <= 128 ? 128 : SETS * COLUMNS <= 256 ? 256 : 512;
-    static constexpr int MISC = STAGES * STAGE;
-    static constexpr int SMEM = MISC + 256;
-    static_assert(STAGES >= 2 && COLUMNS <= 512, "tile");
+    static constexpr int WIDTH = MODE == LINEAR ? TN : 2 * TN;            // columns of what a product of one block fills at most
+    static constexpr bool SHARED_SET = NP == 1 && MODE == GLU_BACKWARD;   // one set, two of dh behind it
+    static constexpr int SETS = SHARED_SET ? 1 : 2;
+    static constexpr int USED = SHARED_SET ? 4 * TN : 2 * WIDTH;
+    static constexpr int TMEM = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+    static constexpr int MISC = STAGES * STAGE, BIAS = MISC + 256;
+    static constexpr int SMEM = BIAS + EPILOGUE_WARPS * 128;
+    static_assert(STAGES >= 2 && USED <= 512 && WIDTH <= 256, "tile");
 };
 
 // ---- activations: value and derivative ---------------------------------------------------------------------------------------
@@ -88,7 +98,7 @@ template <int ACT>
 __device__ __forceinline__ Gate gate_of(float g)
 {
     if constexpr (ACT == SILU) {
-        const float p = 1.f / (1.f + expf(-g));
+        const float p = __fdividef(1.f, 1.f + expf(-g));
         return {g * p, p * (1.f + g * (1.f - p))};
     } else if constexpr (ACT == GELU) {
         const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
@@ -111,46 +121,46 @@ __device__ __forceinline__ void split_words(float a, float b, uint32_t (&w)[3])
     }
 }
 
-// 16 neighbours of a row into its planes; `room` columns from the first one on have memory (a multiple of eight).
+// 16 neighbours of a row into its planes (32 bytes of each: a sector).
 template <class T>
-__device__ __forceinline__ void store_planes(const Planes &to, long long row, int col, int room, const float (&v)[16])
+__device__ __forceinline__ void store_planes(const Planes &to, long long row, int col, const float (&v)[16])
 {
     constexpr int NP = pieces_of<T>;
     using P = typename Piece<T>::type;
     P *at = static_cast<P *>(to.base) + row * to.ld + col;
+    uint32_t w[NP][8];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        if (8 * half >= room) break;
-        uint32_t w[NP][4];
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (NP == 3) {
+            uint32_t s[3];
+            split_words(v[2 * i], v[2 * i + 1], s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = v[8 * half + 2 * i], b = v[8 * half + 2 * i + 1];
-            if constexpr (NP == 3) {
-                uint32_t s[3];
-                split_words(a, b, s);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) w[p][i] = s[p];
-            } else {
-                w[0][i] = pack_two<P>(a, b);
-            }
+            for (int p = 0; p < 3; ++p) w[p][i] = s[p];
+        } else {
+            w[0][i] = pack_two<P>(v[2 * i], v[2 * i + 1]);
         }
-#pragma unroll
-        for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4 *>(at + p * to.plane + 8 * half) = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
     }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) store_32(at + p * to.plane, w[p]);
 }
 
-// 16 neighbours of a row of a matrix of any alignment; `room` of them exist.
+// 16 neighbours of a row of a matrix of any alignment (`wide`: on 32 bytes); `room` of them exist.
 template <class T>
 __device__ __forceinline__ void store_run(T *to, int room, bool wide, const float (&v)[16])
 {
-    constexpr int VEC = 16 / sizeof(T);
     if (wide && room >= 16) {
+        uint32_t w[8];
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 16; i += VEC) {
-            float w[VEC];
+            for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) w[e] = v[i + e];
-            store_values<T, VEC>(to + i, w);
+                for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * half + i]);
+                store_32(to + 8 * half, w);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = pack_two<T>(v[2 * i], v[2 * i + 1]);
+            store_32(to, w);
         }
     } else {
 #pragma unroll
@@ -159,23 +169,46 @@ __device__ __forceinline__ void store_run(T *to, int room, bool wide, const floa
     }
 }
 
+// A lane's bias of 16 columns: of the first (lanes 0 to 15) and the second vector.
 template <class T>
-__device__ __forceinline__ void add_bias(const void *bias, int col, int room, float (&v)[16])
+__device__ __forceinline__ float lane_bias(const void *first, const void *second, int col, int N, int lane)
 {
-    if (bias == nullptr) return;
-    const T *b = static_cast<const T *>(bias) + col;
+    const T *b = static_cast<const T *>(lane < 16 ? first : second);
+    const int at = col + (lane & 15);
+    return b != nullptr && at < N ? to_float(b[at]) : 0.f;
+}
+__device__ __forceinline__ void add_16(const float *b, float (&v)[16])
+{
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i < room) v[i] += to_float(b[i]);
+    for (int i = 0; i < 4; ++i) {
+        const float4 w = reinterpret_cast<const float4 *>(b)[i];
+        v[4 * i] += w.x; v[4 * i + 1] += w.y; v[4 * i + 2] += w.z; v[4 * i + 3] += w.w;
+    }
 }
 
-// The epilogue of 16 columns of one row: v[acc][.] are the accumulators' values.
-template <class T, int MODE, int ACT>
-__device__ __forceinline__ void finish_glu(const Params &p, long long row, int col, float (&v)[MODE == GLU_FORWARD ? 2 : 3][16])
+// Sums of 16 columns over a warp's 32 rows by halving: lanes 2 c and 2 c + 1 end with column c.
+__device__ __forceinline__ float column_sum(const float (&v)[16], int lane)
 {
-    const int room = p.N - col;
-    add_bias<T>(p.bias_gate, col, room, v[0]);
-    add_bias<T>(p.bias_up, col, room, v[1]);
+    float a[8], b[4], c[2];
+    const bool b4 = lane & 16, b3 = lane & 8, b2 = lane & 4, b1 = lane & 2;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (b4 ? v[8 + i] : v[i]) + __shfl_xor_sync(FULL, b4 ? v[i] : v[8 + i], 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = (b3 ? a[4 + i] : a[i]) + __shfl_xor_sync(FULL, b3 ? a[i] : a[4 + i], 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c[i] = (b2 ? b[2 + i] : b[i]) + __shfl_xor_sync(FULL, b2 ? b[i] : b[2 + i], 4);
+    const float d = (b1 ? c[1] : c[0]) + __shfl_xor_sync(FULL, b1 ? c[0] : c[1], 2);
+    return d + __shfl_xor_sync(FULL, d, 1);
+}
+
+// The epilogue of 16 columns of a warp's 32 rows: v[acc][.] are the accumulators' values of this lane's row.
+template <class T, int MODE, int ACT>
+__device__ __forceinline__ void finish_glu(const Params &p, long long row, int col, const float *bias, float (&v)[MODE == GLU_FORWARD ? 2 : 3][16])
+{
+    if (bias != nullptr) {
+        add_16(bias, v[0]);
+        add_16(bias + 16, v[1]);
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const Gate a = gate_of<ACT>(v[0][i]);
@@ -187,35 +220,48 @@ __device__ __forceinline__ void finish_glu(const Params &p, long long row, int c
         }
         v[0][i] = a.a * u;
     }
-    if (row >= p.M) return;
-    store_planes<T>(p.h, row, col, p.padded - col, v[0]);
     if constexpr (MODE == GLU_BACKWARD) {
-        store_planes<T>(p.du, row, col, p.padded - col, v[1]);
-        store_planes<T>(p.dg, row, col, p.padded - col, v[2]);
+        if (p.sums != nullptr) {
+            const int lane = threadIdx.x & 31;
+            const float du = column_sum(v[1], lane), dg = column_sum(v[2], lane);  // (rows behind the last have dh = 0)
+            float *to = p.sums + (row >> 5) * (2ll * p.padded) + col + (lane >> 1);
+            if ((lane & 1) == 0 && (row & ~31ll) < p.M) {
+                to[0] = dg;
+                to[p.padded] = du;
+            }
+        }
+    }
+    if (row >= p.M) return;
+    store_planes<T>(p.h, row, col, v[0]);
+    if constexpr (MODE == GLU_BACKWARD) {
+        store_planes<T>(p.du, row, col, v[1]);
+        store_planes<T>(p.dg, row, col, v[2]);
     }
 }
 
 template <class T, int MODE, int COUNT>
-__device__ __forceinline__ void finish(const Params &p, int split, long long row, int col, float (&v)[COUNT][16])
+__device__ __forceinline__ void finish(const Params &p, int split, long long row, int col, const float *bias, float (&v)[COUNT][16])
 {
     if (col >= p.N) return;
     if constexpr (MODE == LINEAR) {
         if (row >= p.M) return;
         const int room = p.N - col;
         if (p.partial != nullptr) {
-            store_run<float>(p.partial + ((long long)split * p.M + row) * p.N + col, room, (p.N & 3) == 0, v[0]);
+            float *to = p.partial + ((long long)split * p.M + row) * p.N + col;
+            store_run<float>(to, room, (reinterpret_cast<uintptr_t>(to) & 31) == 0, v[0]);
             return;
         }
-        add_bias<T>(p.bias, col, room, v[0]);
+        if (bias != nullptr) add_16(bias, v[0]);
         T *to;
         if (row < p.rows0) to = static_cast<T *>(p.out0) + row * p.ld_out;
         else if (row >= p.row1 && row < p.row1 + p.rows1) to = static_cast<T *>(p.out1) + (row - p.row1) * p.ld_out;
         else return;
-        store_run<T>(to + col, room, ((reinterpret_cast<uintptr_t>(to) & 15) | (p.ld_out & (16 / sizeof(T) - 1))) == 0, v[0]);
+        to += col;
+        store_run<T>(to, room, (reinterpret_cast<uintptr_t>(to) & 31) == 0, v[0]);
     } else {
-        if (p.act == SILU) finish_glu<T, MODE, SILU>(p, row, col, v);
-        else if (p.act == GELU) finish_glu<T, MODE, GELU>(p, row, col, v);
-        else finish_glu<T, MODE, RELU>(p, row, col, v);
+        if (p.act == SILU) finish_glu<T, MODE, SILU>(p, row, col, bias, v);
+        else if (p.act == GELU) finish_glu<T, MODE, GELU>(p, row, col, bias, v);
+        else finish_glu<T, MODE, RELU>(p, row, col, bias, v);
     }
 }
 
@@ -236,37 +282,45 @@ __device__ __forceinline__ Tile tile_of(const Params &p, long long t)
     return x;
 }
 
-template <class T, int MODE, int TN>
+template <class T, int MODE, int TN, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Params p)
 {
     using namespace tc5;
-    using S = Shape<T, MODE, TN>;
+    using S = Shape<T, MODE, TN, PAIR>;
     constexpr int NP = S::NP, STAGES = S::STAGES, SETS = S::SETS;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t base = smem_u32(smem), misc = base + S::MISC;
     volatile unsigned *gave_up = reinterpret_cast<volatile unsigned *>(smem + S::MISC + 240);
-    auto full = [&](int s) { return misc + 8u * (uint32_t)s; };
-    auto empty = [&](int s) { return misc + 64u + 8u * (uint32_t)s; };
-    auto ready = [&](int b) { return misc + 128u + 8u * (uint32_t)b; };
-    auto taken = [&](int b) { return misc + 144u + 8u * (uint32_t)b; };
+    auto full = [&](int s) { return misc + 8u * (uint32_t)s; };        // of a pair: the first block's
+    auto empty = [&](int s) { return misc + 64u + 8u * (uint32_t)s; };  // either block's
+    auto ready = [&](int b) { return misc + 128u + 8u * (uint32_t)b; };  // either block's
+    auto taken = [&](int b) { return misc + 144u + 8u * (uint32_t)b; };  // the first block's
     const uint32_t drained = misc + 160u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_rank() : 0u;
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
-        for (int b = 0; b < SETS; ++b) { mbar_init(ready(b), 1); mbar_init(taken(b), EPILOGUE_WARPS); }
+        for (int b = 0; b < SETS; ++b) { mbar_init(ready(b), 1); mbar_init(taken(b), PAIR ? 2 * EPILOGUE_WARPS : EPILOGUE_WARPS); }
         mbar_init(drained, 1);
         *gave_up = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
     }
-    if (warp == EPILOGUE_WARPS) tmem_alloc<S::TMEM>(misc + 232);
+    if (warp == EPILOGUE_WARPS) {
+        if constexpr (PAIR) tmem_alloc_pair<S::TMEM>(misc + 232);
+        else tmem_alloc<S::TMEM>(misc + 232);
+    }
     fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::MISC + 232);
     grid_launch_dependents();
     grid_dependency_wait();
     const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
+    const long long first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
+    // whether a block of the contraction multiplies with both projections
+    auto is_gu = [&](int kb) { return MODE == GLU_FORWARD || (MODE == GLU_BACKWARD && kb >= p.blocks0); };
 
     if (warp == EPILOGUE_WARPS + 1) {
         // ---- copies ----
@@ -275,40 +329,49 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             uint32_t phase = 1;
             bool ok = true;
             long long sent = 0;
+            auto box = [&](uint32_t to, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+                if constexpr (PAIR) tma_load_3d_pair(to, map, x, y, z, bar);
+                else tma_load_3d(to, map, x, y, z, bar);
+            };
             auto operand = [&](const CUtensorMap *map, bool across, uint32_t to, int rows, int row, int k, int piece, uint32_t bar) {
                 if (!across) {
-                    tma_load_3d(to, map, k, row, piece, bar);
+                    box(to, map, k, row, piece, bar);
                 } else {
-                    for (int i = 0; i < rows; i += 64) tma_load_3d(to + i * 128u, map, row + i, k, piece, bar);
+                    for (int i = 0; i < rows; i += 64) box(to + i * 128u, map, row + i, k, piece, bar);
                 }
             };
-            for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (long long t = first_tile; t < tiles && ok; t += stride) {
                 const Tile x = tile_of(p, t);
+                const int m0 = (PAIR ? 2 * x.m + (int)rank : x.m) * TM, n0 = x.n * TN;
                 for (int kb = x.k_lo; kb < x.k_hi; ++kb) {
                     ok = mbar_wait(empty(s), phase, gave_up);
                     if (!ok) break;
                     const int part = kb >= p.blocks0, k = (part ? kb - p.blocks0 : kb) * TK;
+                    const bool gu = is_gu(kb);
                     const uint32_t at = base + s * S::STAGE, bt = at + NP * S::A_PIECE;
-                    const bool two = MODE != LINEAR && part == 0;  // gate and up
-                    mbar_expect(full(s), (uint32_t)(NP * (S::A_PIECE + (two ? 2 : 1) * TN * TK * 2)));
+                    const uint32_t bar = PAIR ? mapa(full(s), 0) : full(s);
+                    if (rank == 0)
+                        mbar_expect(full(s), (uint32_t)((PAIR ? 2 : 1) * NP * (S::A_PIECE + (gu ? S::ROWS_GU : S::ROWS_ONE) * TK * 2)));
 #pragma unroll
                     for (int i = 0; i < NP; ++i) {
-                        operand(&p.a[part], p.a_across[part], at + i * S::A_PIECE, TM, x.m * TM, k, i, full(s));
+                        operand(&p.a[part], p.a_across[part], at + i * S::A_PIECE, TM, m0, k, i, bar);
                         const uint32_t bi = bt + i * S::B_PIECE;
-                        if (MODE == LINEAR) {
-                            operand(&p.b[part], p.b_across[part], bi, TN, x.n * TN, k, i, full(s));
-                        } else if (part == 0) {
-                            operand(&p.b[0], p.b_across[0], bi, TN, x.n * TN, k, i, full(s));
-                            operand(&p.b[1], p.b_across[0], bi + TN * TK * 2, TN, x.n * TN, k, i, full(s));
+                        if (gu) {
+                            if (PAIR) {
+                                operand(&p.b[1 + rank], false, bi, TN, n0, k, i, bar);
+                            } else {
+                                operand(&p.b[1], false, bi, TN, n0, k, i, bar);
+                                operand(&p.b[2], false, bi + TN * TK * 2, TN, n0, k, i, bar);
+                            }
                         } else {
-                            operand(&p.b[2], p.b_across[1], bi, TN, x.n * TN, k, i, full(s));
+                            operand(&p.b[part], p.b_across[part], bi, S::ROWS_ONE, n0 + (int)rank * S::ROWS_ONE, k, i, bar);
                         }
                     }
                     ++sent;
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
             }
-            if (!ok) {  // the copies in flight land before the block goes: the last of each stage
+            if (!ok && rank == 0) {  // the copies in flight land before the block goes (and its pair: the cluster leaves together)
                 unsigned mine = 0u;
                 for (int i = 0; i < STAGES && i < sent; ++i) {
                     if (--s < 0) { s = STAGES - 1; phase ^= 1u; }
@@ -318,16 +381,27 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         }
     } else if (warp == EPILOGUE_WARPS) {
         // ---- products ----
-        if (lane == 0) {
-            constexpr int AB = sizeof(typename Piece<T>::type) == 2 && !std::is_same<typename Piece<T>::type, __half>::value ? 1 : 0;
-            int s = 0, b = 0;
+        if (lane == 0 && rank == 0) {
+            constexpr int AB = std::is_same<typename Piece<T>::type, __half>::value ? 0 : 1, IM = PAIR ? 2 * TM : TM;
+            auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+                if constexpr (PAIR) mma_f16_pair(d, a, b, idesc, accumulate);
+                else mma_f16(d, a, b, idesc, accumulate);
+            };
+            auto commit = [&](uint32_t bar) {
+                if constexpr (PAIR) mma_commit_pair(bar);
+                else mma_commit(bar);
+            };
+            int s = 0, b = 0, dh_set = 0;
             uint32_t phase = 0, set_phase = 1;
             bool ok = true;
-            for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+            for (long long t = first_tile; t < tiles && ok; t += stride) {
                 const Tile x = tile_of(p, t);
                 for (int kb = x.k_lo; kb < x.k_hi; ++kb) {
-                    const bool fresh = NP > 1 || kb == x.k_lo;  // the first block of its accumulators
-                    if (fresh) {
+                    const int part = kb >= p.blocks0;
+                    const bool gu = is_gu(kb);
+                    const bool clear = NP > 1 || kb == x.k_lo || (MODE == GLU_BACKWARD && kb == p.blocks0);  // the first block of an accumulator
+                    // (where the sets of dh lie behind a shared one, that of the tile before last has been taken: see the wait below)
+                    if (clear && (!S::SHARED_SET || gu)) {
                         ok = mbar_wait(taken(b), set_phase, gave_up);
                         if (!ok) break;
                         fence_after();
@@ -335,12 +409,9 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     ok = mbar_wait(full(s), phase, gave_up);
                     if (!ok) break;
                     fence_after();
-                    const int part = kb >= p.blocks0;
-                    const bool two = MODE != LINEAR && part == 0;
-                    const uint32_t d = tmem + b * S::COLUMNS + (MODE == GLU_BACKWARD && part ? 2 * TN : 0);
-                    const bool clear = fresh || (MODE == GLU_BACKWARD && kb == p.blocks0);
-                    const bool aa = p.a_across[part], ba = p.b_across[part];
-                    const uint32_t idesc = (two ? instr_desc<TM, 2 * TN <= 256 ? 2 * TN : 256, AB, false>() : instr_desc<TM, TN, AB, false>()) |
+                    const uint32_t d = tmem + (S::SHARED_SET ? (gu ? 0u : (2u + dh_set) * TN) : (uint32_t)(b * S::WIDTH));
+                    const bool aa = p.a_across[part], ba = !gu && p.b_across[part];
+                    const uint32_t idesc = (gu ? instr_desc<IM, MODE == LINEAR ? TN : 2 * TN, AB, false>() : instr_desc<IM, TN, AB, false>()) |
                                            (aa ? 1u << 15 : 0u) | (ba ? 1u << 16 : 0u);
                     // a step of 16 along the contraction: 32 bytes of a row, or 16 rows; panels of 64 across it lie 8 KB apart
                     const uint32_t a_step = (aa ? 2048 : 32) >> 4, b_step = (ba ? 2048 : 32) >> 4;
@@ -349,50 +420,72 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     constexpr uint32_t AP = S::A_PIECE >> 4, BP = S::B_PIECE >> 4;
                     if constexpr (NP == 1) {
 #pragma unroll
-                        for (int ks = 0; ks < TK / 16; ++ks) mma_f16(d, a0 + ks * a_step, b0 + ks * b_step, idesc, !(clear && ks == 0));
+                        for (int ks = 0; ks < TK / 16; ++ks) mma(d, a0 + ks * a_step, b0 + ks * b_step, idesc, !(clear && ks == 0));
                     } else {
 #pragma unroll
                         for (int ks = 0; ks < TK / 16; ++ks) {
                             const uint64_t ak = a0 + ks * a_step, bk = b0 + ks * b_step;
-                            mma_f16(d, ak + 2 * AP, bk, idesc, ks > 0);
-                            mma_f16(d, ak, bk + 2 * BP, idesc, true);
-                            mma_f16(d, ak + AP, bk + BP, idesc, true);
+                            mma(d, ak + 2 * AP, bk, idesc, ks > 0);
+                            mma(d, ak, bk + 2 * BP, idesc, true);
+                            mma(d, ak + AP, bk + BP, idesc, true);
                         }
 #pragma unroll
                         for (int ks = 0; ks < TK / 16; ++ks) {
                             const uint64_t ak = a0 + ks * a_step, bk = b0 + ks * b_step;
-                            mma_f16(d, ak + AP, bk, idesc, true);
-                            mma_f16(d, ak, bk + BP, idesc, true);
+                            mma(d, ak + AP, bk, idesc, true);
+                            mma(d, ak, bk + BP, idesc, true);
                         }
 #pragma unroll
-                        for (int ks = 0; ks < TK / 16; ++ks) mma_f16(d, a0 + ks * a_step, b0 + ks * b_step, idesc, true);
+                        for (int ks = 0; ks < TK / 16; ++ks) mma(d, a0 + ks * a_step, b0 + ks * b_step, idesc, true);
                     }
-                    mma_commit(empty(s));
+                    commit(empty(s));
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                     if (NP > 1 || kb == x.k_hi - 1) {
-                        mma_commit(ready(b));
+                        commit(ready(b));
                         if (++b == SETS) { b = 0; set_phase ^= 1u; }
                     }
                 }
+                dh_set ^= 1;
             }
             if (!ok) {  // the instructions issued so far
                 unsigned mine = 0u;
-                mma_commit(drained);
+                commit(drained);
                 mbar_wait(drained, 0, &mine);
             }
         }
     } else {
-        // ---- epilogue: warp w has rows 32 (w % 4) .. + 31 of the tile and half of its columns ----
-        constexpr int CHUNKS = TN / 32;  // of 16 columns
-        const int first = (warp >> 2) * (TN / 2);
+        // ---- epilogue: warp w has rows 32 (w % 4) .. + 31 of the tile and a quarter of its columns ----
+        constexpr int SHARE = TN / (EPILOGUE_WARPS / 4), CHUNKS = SHARE / 16;
+        const int first = (warp >> 2) * SHARE;
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + first;
-        int b = 0;
+        float *bias_16 = reinterpret_cast<float *>(smem + S::BIAS) + warp * 32;
+        const void *bias_a = MODE == LINEAR ? p.bias : p.bias_gate, *bias_b = MODE == LINEAR ? nullptr : p.bias_up;
+        const bool biased = bias_a != nullptr || bias_b != nullptr;
+        auto give_back = [&](int b) {
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_at(mapa(taken(b), 0));
+                else mbar_arrive(taken(b));
+            }
+        };
+        int b = 0, dh_set = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for (long long t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (long long t = first_tile; t < tiles && ok; t += stride) {
             const Tile x = tile_of(p, t);
-            const long long row = (long long)x.m * TM + (warp & 3) * 32 + lane;
+            const long long row = ((long long)(PAIR ? 2 * x.m + rank : x.m)) * TM + (warp & 3) * 32 + lane;
             const int col = x.n * TN + first;
+            float bias[CHUNKS];
+#pragma unroll
+            for (int c = 0; c < CHUNKS; ++c) bias[c] = biased ? lane_bias<T>(bias_a, bias_b, col + c * 16, p.N, lane) : 0.f;
+            auto place_bias = [&](int c) -> const float * {
+                if (!biased) return nullptr;
+                __syncwarp();
+                bias_16[lane] = bias[c];
+                __syncwarp();
+                return bias_16;
+            };
             if constexpr (NP == 1) {
                 ok = mbar_wait(ready(b), phase, gave_up);
                 ok = __all_sync(FULL, ok);
@@ -401,15 +494,14 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c) {
                     float v[S::ACCS][16];
-                    tmem_load_rows16<S::ACCS>(lanes + b * S::COLUMNS + c * 16, TN, v);
-                    if (c == CHUNKS - 1) {
-                        fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(taken(b));
-                    }
-                    finish<T, MODE>(p, x.split, row, col + c * 16, v);
+                    const uint32_t at = lanes + b * S::WIDTH + c * 16;
+                    // (dh is the third accumulator: two or three widths behind the first)
+                    tmem_load_rows16<S::ACCS>(at, TN, v, S::SHARED_SET ? dh_set * TN : 0);
+                    if (c == CHUNKS - 1) give_back(b);
+                    finish<T, MODE>(p, x.split, row, col + c * 16, place_bias(c), v);
                 }
                 if (++b == SETS) { b = 0; phase ^= 1u; }
+                dh_set ^= 1;
             } else {
                 float sum[CHUNKS][S::ACCS][16];
 #pragma unroll
@@ -423,12 +515,12 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     ok = __all_sync(FULL, ok);
                     if (!ok) break;
                     fence_after();
-                    const uint32_t at = lanes + b * S::COLUMNS;
-                    if (MODE == GLU_BACKWARD && kb >= p.blocks0) {
+                    const uint32_t at = lanes + b * S::WIDTH;
+                    if (MODE == GLU_BACKWARD && kb < p.blocks0) {
 #pragma unroll
                         for (int c = 0; c < CHUNKS; ++c) {
                             float v[1][16];
-                            tmem_load_rows16<1>(at + 2 * TN + c * 16, TN, v);
+                            tmem_load_rows16<1>(at + c * 16, TN, v, 0);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) sum[c][S::ACCS - 1][i] += v[0][i];
                         }
@@ -437,28 +529,30 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 #pragma unroll
                         for (int c = 0; c < CHUNKS; ++c) {
                             float v[NOW][16];
-                            tmem_load_rows16<NOW>(at + c * 16, TN, v);
+                            tmem_load_rows16<NOW>(at + c * 16, TN, v, 0);
 #pragma unroll
                             for (int a = 0; a < NOW; ++a)
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) sum[c][a][i] += v[a][i];
                         }
                     }
-                    fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(taken(b));
+                    give_back(b);
                     if (++b == SETS) { b = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c) finish<T, MODE>(p, x.split, row, col + c * 16, sum[c]);
+                for (int c = 0; c < CHUNKS; ++c) finish<T, MODE>(p, x.split, row, col + c * 16, place_bias(c), sum[c]);
             }
         }
     }
     fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();
     fence_after();
-    if (warp == EPILOGUE_WARPS) tmem_free<S::TMEM>(tmem);
+    if (warp == EPILOGUE_WARPS) {
+        if constexpr (PAIR) tmem_free_pair<S::TMEM>(tmem);
+        else tmem_free<S::TMEM>(tmem);
+    }
     if (threadIdx.x == 0) report_waits(gave_up, p.status);
 }
 

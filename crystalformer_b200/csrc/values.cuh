@@ -84,6 +84,14 @@ __device__ __forceinline__ void store_values(T *p, const float (&v)[VEC])
     }
 }
 
+// 32 neighbouring bytes, aligned to that, in one store
+__device__ __forceinline__ void store_32(void *p, const uint32_t (&w)[8])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
 inline bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 }  // namespace cf
