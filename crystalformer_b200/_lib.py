@@ -215,3 +215,21 @@ def call(name: str, *args) -> None:
     code = getattr(lib, name)(*args)
     if code != 0:
         raise CrystalformerB200Error(name, code, lib.cf_last_error().decode())
+
+
+_torch_ops = None
+
+
+def torch_ops():
+    """The torch functions of ``csrc/torch_binding.cpp``; raises if they have not been built."""
+    global _torch_ops
+    if _torch_ops is None:
+        load()
+        import torch  # noqa: F401  (its libraries are what the module is linked to)
+        try:
+            from . import _torch_ops as module
+        except ImportError as e:
+            raise ImportError("crystalformer_b200/_torch_ops.so is missing or belongs to another torch: build it with "
+                              "`python -m crystalformer_b200.build`") from e
+        _torch_ops = module
+    return _torch_ops

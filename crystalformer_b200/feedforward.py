@@ -8,27 +8,13 @@ from __future__ import annotations
 
 from typing import Optional
 
-import torch
 from torch import Tensor
 from torch.nn import Linear, Module
 
-from . import ops
+from . import _lib, ops
 
 #: activation of the encoder -> of the gate
 GATES = {"swiglu": "silu", "geglu": "gelu", "reglu": "relu"}
-
-
-class GatedFeedForwardFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation: str):
-        ctx.save_for_backward(x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-        ctx.activation = activation
-        return ops.gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy):
-        return (*ops.gated_ffn_bwd(*ctx.saved_tensors, ctx.activation, gy, ctx.needs_input_grad[:7]), None)
 
 
 def gated_feed_forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, b_gate: Optional[Tensor] = None, b_up: Optional[Tensor] = None,
@@ -37,15 +23,7 @@ def gated_feed_forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, 
     x (..., D); ``activation``: "silu", "gelu" (the exact one) or "relu".  All of one type; of any sizes.  float32 has float32's
     accuracy (operands in three pieces on the tensor cores); of 16-bit types the hidden features and their gradients are rounded to
     the type once, sums are float32.  The backward computes the hidden features again instead of keeping them."""
-    shape = x.shape
-    if x.dim() != 2:
-        x = x.reshape(-1, shape[-1]) if x.dim() > 0 else x
-    leaves = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves):
-        y = GatedFeedForwardFunction.apply(*leaves, activation)
-    else:
-        y = ops.gated_ffn_fwd(*leaves, activation)
-    return y if len(shape) == 2 else y.view(shape)
+    return _lib.torch_ops().gated(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.gate_code(activation))
 
 
 class GatedFeedForward(Module):

@@ -6,7 +6,7 @@ fused attention module; they have no CPU path.
 """
 from __future__ import annotations
 
-from ctypes import byref, c_double, c_int, c_int64, c_void_p
+from ctypes import c_double, c_int, c_int64, c_void_p
 from typing import Optional, Tuple
 
 import torch
@@ -541,188 +541,46 @@ def pipe_probe(kind: int, blocks: int, threads: int, iters: int, sink: torch.Ten
 
 
 # ---------------------------------------------------------------------------------------------------------------------
-# Operators of an encoder layer beside the attention, in float32, bfloat16 and float16 (inputs and outputs of one type)
+# Operators of an encoder layer beside the attention, in float32, bfloat16 and float16 (inputs and outputs of one type),
+# without autograd (embedding.py, qk_norm.py and feedforward.py have it); checks and launches are in csrc/torch_binding.cpp.
 # ---------------------------------------------------------------------------------------------------------------------
-TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # CF_FLOAT32, CF_BFLOAT16, CF_FLOAT16
+GATE_CODES = {"silu": 0, "gelu": 1, "relu": 2}  # CF_GATE_SILU, CF_GATE_GELU, CF_GATE_RELU
 
 
-def _call_on(device: torch.device, name: str, *args) -> None:
-    """The call with `device` current and its current stream as the last argument."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
-
-
-def _like(t: Optional[torch.Tensor], first: torch.Tensor, name: str, shape) -> None:
-    """Checks that `t` is there, lies where `first` does, with its type and the shape given."""
-    if t is None:
-        return
-    if t.device != first.device:
-        raise RuntimeError(f"{name} is on {t.device}, expected {first.device}")
-    if t.dtype != first.dtype:
-        raise TypeError(f"{name} must be {first.dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have the shape {tuple(shape)}, got {tuple(t.shape)}")
-
-
-def _first(t: torch.Tensor, name: str, dims: int) -> torch.Tensor:
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor: crystalformer_b200 has no CPU path")
-    if t.dtype not in TYPE_CODES:
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dimensions, got the shape {tuple(t.shape)}")
-    return t
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t, copied unless the entries of its rows are neighbours."""
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 and t.is_contiguous() else t.contiguous()
-
-
-def _ids(ids: torch.Tensor, device) -> torch.Tensor:
-    if ids.device != device:
-        raise RuntimeError(f"ids are on {ids.device}, expected {device}")
-    if ids.dtype != torch.int64:
-        if ids.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
-            raise TypeError(f"ids must be whole numbers, got {ids.dtype}")
-        ids = ids.to(torch.int64)
-    return ids if ids.is_contiguous() else ids.contiguous()
+def gate_code(activation: str) -> int:
+    code = GATE_CODES.get(activation)
+    if code is None:
+        raise ValueError(f"activation {activation!r} is none of {', '.join(GATE_CODES)}")
+    return code
 
 
 def embed_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * table[ids], (*ids.shape, D); ids outside the table give rows of zeros.  ``table`` (V,D) may have any strides."""
-    table = _first(table, "table", 2)
-    ids = _ids(ids, table.device)
-    V, D = table.shape
-    out = torch.empty((*ids.shape, D), dtype=table.dtype, device=table.device)
-    _call_on(table.device, "cf_embed_fwd", table.data_ptr(), table.stride(0), table.stride(1), TYPE_CODES[table.dtype], ids.data_ptr(), ids.numel(),
-             V, D, scale, out.data_ptr())
-    return out
+    return _lib.torch_ops().embed_fwd(ids, table, scale)
 
 
 def embed_bwd(ids: torch.Tensor, gout: torch.Tensor, V: int, scale: float = 1.0, transposed: bool = False) -> torch.Tensor:
     """The gradient (V,D) of the table of ``embed_fwd`` from that of its output; ``transposed``: a view of a (D,V) contiguous tensor."""
-    if not gout.is_cuda:
-        raise RuntimeError("gout must be a CUDA tensor: crystalformer_b200 has no CPU path")
-    dev, D = gout.device, gout.shape[-1]
-    ids = _ids(ids, dev)
-    if tuple(gout.shape[:-1]) != tuple(ids.shape):
-        raise ValueError(f"gout {tuple(gout.shape)} does not belong to ids {tuple(ids.shape)}")
-    gout = _first(gout.reshape(-1, D), "gout", 2)
-    gout = _rows(gout)
-    N = ids.numel()
-    gtable = torch.empty((D, V) if transposed else (V, D), dtype=gout.dtype, device=dev)
-    work = torch.empty(int(_lib.load().cf_embed_bwd_workspace_bytes(N, D)), dtype=torch.uint8, device=dev)
-    _call_on(dev, "cf_embed_bwd", gout.data_ptr(), gout.stride(0) if N > 1 else D, TYPE_CODES[gout.dtype], ids.data_ptr(), N, V, D, scale,
-             gtable.data_ptr(), int(transposed), work.data_ptr())
-    return gtable.t() if transposed else gtable
-
-
-def _qk_args(q, k, wq, wk, pos, waves, eps: float, interleaved: bool):
-    """The description of a call, and the tensors that it points into."""
-    q, k = _first(q, "q", 3), _first(k, "k", 3)
-    N, Hq, D = q.shape
-    Hk = k.shape[1]
-    _like(k, q, "k", (N, Hk, D))
-    q, k = _rows(q), _rows(k)
-    heads = []
-    for name, w, H in (("wq", wq, Hq), ("wk", wk, Hk)):
-        _like(w, q, name, (H, D) if w is not None and w.dim() == 2 else (D,))
-        heads.append(None if w is None else w.contiguous())
-    wq, wk = heads
-    P = C = 0
-    wave_heads = 1
-    if waves is not None:
-        if waves.dim() != 3 or pos is None or pos.dim() != 2 or pos.shape != (N, waves.shape[2]):
-            raise ValueError(f"waves (heads, pairs, axes) and pos (rows, axes) go together: got {tuple(waves.shape)} and "
-                             f"{None if pos is None else tuple(pos.shape)} for {N} rows")
-        pos, waves = _want(pos, torch.float32, "pos", q.device), _want(waves, torch.float32, "waves", q.device)
-        wave_heads, P, C = waves.shape
-    elif pos is not None:
-        raise ValueError("positions without waves")
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    args = _lib.QkNorm(TYPE_CODES[q.dtype], int(interleaved), N, Hq, Hk, D, P, C, wave_heads, ptr(q), q.stride(0), q.stride(1), ptr(k), k.stride(0),
-                       k.stride(1), ptr(wq), D if wq is not None and wq.dim() == 2 else 0, ptr(wk), D if wk is not None and wk.dim() == 2 else 0,
-                       ptr(pos), ptr(waves), eps)
-    return args, (q, k, wq, wk, pos, waves)
+    return _lib.torch_ops().embed_bwd(ids, gout, V, scale, transposed)
 
 
 def qk_norm_fwd(q, k, wq=None, wk=None, pos=None, waves=None, eps: float = 1e-6, interleaved: bool = False):
     """Norms of the heads of q (N,Hq,D) and k (N,Hk,D), times the weights, then the rotation by positions (cf_qk_norm_fwd)."""
-    args, keep = _qk_args(q, k, wq, wk, pos, waves, eps, interleaved)
-    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in keep[:2])
-    _call_on(q.device, "cf_qk_norm_fwd", byref(args), q_out.data_ptr(), k_out.data_ptr())
-    return q_out, k_out
+    with torch.no_grad():
+        return _lib.torch_ops().normalize_rotate(q, k, wq, wk, pos, waves, eps, interleaved)
 
 
 def qk_norm_bwd(q, k, wq, wk, pos, waves, eps: float, interleaved: bool, gq_out, gk_out, want_wq: bool = True, want_wk: bool = True):
     """Gradients (gq, gk, gwq, gwk) of ``qk_norm_fwd``'s inputs; those of absent or unwanted weights are None."""
-    args, keep = _qk_args(q, k, wq, wk, pos, waves, eps, interleaved)
-    _like(gq_out, q, "gq_out", q.shape)
-    _like(gk_out, q, "gk_out", k.shape)
-    gq_out, gk_out = gq_out.contiguous(), gk_out.contiguous()
-    dev = q.device
-    gq, gk = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in keep[:2])
-    gwq, gwk = (None if w is None or not want else torch.empty(w.shape, dtype=w.dtype, device=dev) for w, want in ((wq, want_wq), (wk, want_wk)))
-    work = None
-    if gwq is not None or gwk is not None:
-        with torch.cuda.device(dev):
-            work = torch.empty(int(_lib.load().cf_qk_norm_bwd_workspace_bytes(byref(args))), dtype=torch.uint8, device=dev)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    _call_on(dev, "cf_qk_norm_bwd", byref(args), gq_out.data_ptr(), gk_out.data_ptr(), gq.data_ptr(), gk.data_ptr(), ptr(gwq), ptr(gwk), ptr(work))
-    return gq, gk, gwq, gwk
-
-
-GATE_CODES = {"silu": 0, "gelu": 1, "relu": 2}  # CF_GATE_SILU, CF_GATE_GELU, CF_GATE_RELU
-
-
-def _gated_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation: str):
-    """The description of a call, and the tensors that it points into."""
-    x = _first(x, "x", 2)
-    if activation not in GATE_CODES:
-        raise ValueError(f"activation {activation!r} is none of {', '.join(GATE_CODES)}")
-    N, D = x.shape
-    if w_gate.dim() != 2:
-        raise ValueError(f"w_gate must have 2 dimensions, got the shape {tuple(w_gate.shape)}")
-    F = w_gate.shape[0]
-    for t, name, shape in ((w_gate, "w_gate", (F, D)), (w_up, "w_up", (F, D)), (w_down, "w_down", (D, F)), (b_gate, "b_gate", (F,)),
-                           (b_up, "b_up", (F,)), (b_down, "b_down", (D,))):
-        _like(t, x, name, shape)
-    x = _rows(x)
-    rest = [None if t is None else t if t.is_contiguous() else t.contiguous() for t in (w_gate, w_up, w_down, b_gate, b_up, b_down)]
-    return _lib.GatedFFN(TYPE_CODES[x.dtype], GATE_CODES[activation], N, D, F, x.data_ptr(), x.stride(0) if N > 1 else D,
-                         *[None if t is None else t.data_ptr() for t in rest]), x, rest
-
-
-def _gated_work(args, gy, device, backward: bool):
-    lib, at = _lib.load(), 0 if gy is None else gy.data_ptr()
-    if torch.cuda.current_device() == device.index:
-        nbytes = lib.cf_gated_ffn_workspace_bytes(byref(args), at, int(backward))
-    else:
-        with torch.cuda.device(device):
-            nbytes = lib.cf_gated_ffn_workspace_bytes(byref(args), at, int(backward))
-    return torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+    return _lib.torch_ops().normalize_rotate_backward(q, k, wq, wk, pos, waves, eps, interleaved, gq_out, gk_out, want_wq, want_wk)
 
 
 def gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, activation: str = "silu"):
-    """The gated feed-forward block of x (N,D): see ``feedforward.gated_feed_forward`` (cf_gated_ffn_fwd)."""
-    args, x, keep = _gated_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    work = _gated_work(args, None, x.device, False)
-    _call_on(x.device, "cf_gated_ffn_fwd", byref(args), y.data_ptr(), work.data_ptr())
-    return y
+    """The gated feed-forward block of x (..., D): see ``feedforward.gated_feed_forward`` (cf_gated_ffn_fwd)."""
+    with torch.no_grad():
+        return _lib.torch_ops().gated(x, w_gate, w_up, w_down, b_gate, b_up, b_down, gate_code(activation))
 
 
 def gated_ffn_bwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation: str, gy, wanted=(True,) * 7):
-    """Gradients of ``gated_ffn_fwd``'s seven tensors from that of its output; None where absent or not ``wanted``."""
-    args, x, keep = _gated_args(x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation)
-    _like(gy, x, "gy", x.shape)
-    gy = gy.contiguous()
-    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and want else None for t, want in zip((x, *keep), wanted)]
-    work = _gated_work(args, gy, x.device, True)
-    to = _lib.GatedFFNGrads(gy.data_ptr(), *[None if t is None else t.data_ptr() for t in grads])
-    _call_on(x.device, "cf_gated_ffn_bwd", byref(args), byref(to), work.data_ptr())
-    return tuple(grads)
+    """Gradients of ``gated_ffn_fwd``'s seven tensors (x of two dimensions) from that of its output; None where absent or not ``wanted``."""
+    return tuple(_lib.torch_ops().gated_backward(x, w_gate, w_up, w_down, b_gate, b_up, b_down, gate_code(activation), gy, list(wanted)))

@@ -11,21 +11,7 @@ import torch
 from torch import Tensor
 from torch.nn import Module, Parameter
 
-from . import ops
-
-
-class NormalizeRotateFunction(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, pos, waves, eps: float, interleaved: bool):
-        ctx.save_for_backward(q, k, wq, wk, pos, waves)
-        ctx.how = eps, interleaved
-        return ops.qk_norm_fwd(q, k, wq, wk, pos, waves, eps, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq_out, gk_out):
-        grads = ops.qk_norm_bwd(*ctx.saved_tensors, *ctx.how, gq_out, gk_out, ctx.needs_input_grad[2], ctx.needs_input_grad[3])
-        return (*grads, None, None, None, None)
+from . import _lib
 
 
 def normalize_rotate(q: Tensor, k: Tensor, wq: Optional[Tensor] = None, wk: Optional[Tensor] = None, pos: Optional[Tensor] = None,
@@ -36,9 +22,7 @@ def normalize_rotate(q: Tensor, k: Tensor, wq: Optional[Tensor] = None, wk: Opti
     2 P on are not turned.  Waves count cycles per unit of position and angles keep their accuracy at any distance.  q and k may
     be strided views (of a joint projection); outputs are contiguous, of their type (float32, bfloat16 or float16).  Gradients: of
     q, k and the weights."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)):
-        return NormalizeRotateFunction.apply(q, k, wq, wk, pos, waves, float(eps), bool(interleaved))
-    return ops.qk_norm_fwd(q, k, wq, wk, pos, waves, float(eps), bool(interleaved))
+    return _lib.torch_ops().normalize_rotate(q, k, wq, wk, pos, waves, eps, interleaved)
 
 
 def shortest_waves(heads: int, pairs: int) -> Tensor:

@@ -202,11 +202,12 @@ def test_outputs_end_where_they_end():
     """No kernel writes behind an output: outputs inside larger buffers, their surroundings marked."""
     import ctypes
 
-    from crystalformer_b200 import _lib, ops
+    from crystalformer_b200 import _lib
     for dtype in TYPES:
         for N, D, F in ((3, 33, 17), (130, 33, 17), (130, 72, 136), (2000, 40, 24)):
             tensors, gy = make(N, D, F, dtype)
-            args, x, keep = ops._gated_args(*tensors, "silu")
+            args = _lib.GatedFFN(TYPES.index(dtype), 0, N, D, F, tensors[0].data_ptr(), D, *[t.data_ptr() for t in tensors[1:]])
+            stream = torch.cuda.current_stream().cuda_stream
             shapes = [(N, D)] + [tuple(t.shape) for t in tensors]
             room = [torch.full((torch.Size(s).numel() + 64,), 7.0, dtype=dtype, device="cuda") for s in shapes]
             outs = [r[32:32 + torch.Size(s).numel()] for r, s in zip(room, shapes)]
@@ -216,9 +217,9 @@ def test_outputs_end_where_they_end():
                 assert work.data_ptr() % 256 == 0
                 if back:
                     grads = _lib.GatedFFNGrads(gy.data_ptr(), *[o.data_ptr() for o in outs[1:]])
-                    ops._call_on(x.device, "cf_gated_ffn_bwd", ctypes.byref(args), ctypes.byref(grads), work.data_ptr())
+                    _lib.call("cf_gated_ffn_bwd", ctypes.byref(args), ctypes.byref(grads), work.data_ptr(), stream)
                 else:
-                    ops._call_on(x.device, "cf_gated_ffn_fwd", ctypes.byref(args), outs[0].data_ptr(), work.data_ptr())
+                    _lib.call("cf_gated_ffn_fwd", ctypes.byref(args), outs[0].data_ptr(), work.data_ptr(), stream)
                 torch.cuda.synchronize()
                 assert (work[nbytes:] == 77).all()
             assert all((r[:32] == 7).all() and (r[32 + o.numel():] == 7).all() for r, o in zip(room, outs))

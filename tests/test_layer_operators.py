@@ -103,3 +103,16 @@ def test_options_of_the_layers():
     assert more == {"linear_gate.weight", "linear_gate.bias", "self_attn.qk_norm.q_weight", "self_attn.qk_norm.k_weight", "self_attn.qk_norm.waves"}
     assert set(plain.state_dict()) <= set(layer.state_dict()) and plain.gate is None and plain.self_attn.qk_norm is None
     assert layer.gate == "silu" and layer.self_attn.qk_norm.waves.shape == (8, 8, 3)
+
+
+def test_kinds_of_errors(lib):
+    """What the torch functions throw arrives as Python's own exceptions."""
+    from crystalformer_b200 import ops
+    with pytest.raises(ValueError, match="does not belong"):
+        ops.embed_bwd(torch.zeros(3, dtype=torch.int64), torch.zeros(4, 8), 5)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.embed_bwd(torch.zeros(4, dtype=torch.int64), torch.zeros(4, 8), 5)
+    with pytest.raises(TypeError):
+        ops.embed_bwd(None, torch.zeros(4, 8), 5)
+    with pytest.raises(ValueError):
+        ops.gated_ffn_fwd(torch.zeros(3, 4), torch.zeros(5, 4), torch.zeros(5, 4), torch.zeros(4, 5), activation="tanh")
