@@ -8,12 +8,15 @@
 // Bound by memory (2 + 2 bytes or 4 + 4 a value forward), as long as the sines do not dominate: an angle is computed once per key
 // head and used for that key head and the query heads that share it.  A head is held by the fewest lanes (a power of two) that
 // take it in slots of 2 VEC values - a pair of vectors whose entries are partners - so that sums of squares are a few shuffles and
-// nothing is exchanged for the rotation.  Waves count cycles per unit of position: the products are exact (a rounded product and
-// its fused remainder), whole turns are dropped before the parts are added, and an angle is off by 2^-24 turns however far the
-// position; whole-numbered waves on fractional coordinates thus do not see lattice translations at all.
+// nothing is exchanged for the rotation.  A group of lanes walks the rows with the same heads of each: its weights and waves stay in
+// registers, and the next head's values are on their way while one is computed (without that, and with 16-byte vectors' twice as
+// many registers, the backward of 16,384 rows of 32 + 8 heads of 128 took 353 us).  Waves count cycles per unit of position: the
+// products are exact (a rounded product and its fused remainder), whole turns are dropped before the parts are added, and an angle
+// is off by 2^-24 turns however far the position; whole-numbered waves on fractional coordinates thus do not see lattice
+// translations at all.
 //
-// The weights' gradients are sums over all rows: each lane keeps its entries' in registers while it walks the rows, a block adds
-// its lanes' in a fixed order, and a second kernel adds the blocks'.
+// The weights' gradients are sums over all rows: each lane keeps its entries' in registers, a block adds its lanes' in a fixed order,
+// and a second kernel adds the blocks'.
 #include "common.cuh"
 #include "values.cuh"
 
@@ -26,7 +29,8 @@ struct HeadArgs {
     cf_qk_norm d;
     const void *gq_out, *gk_out;  // backward: gradients of the outputs, (N, H, D) contiguous
     void *q_out, *k_out;          // outputs, or the inputs' gradients
-    float *partial;               // (blocks, units, D) sums of the weights' gradients
+    float *partial;               // (blocks, columns) sums of the weights' gradients: of wq, then of wk, each (1 or H, D)
+    int columns, columns_q;
     int lanes;                    // of a head
     int slots;                    // of a head: 2 VEC values each
     int rotated;                  // slots of rotated values
@@ -34,125 +38,17 @@ struct HeadArgs {
     int single;
 };
 
-template <int VEC>
 struct Place {  // of a slot's two vectors in a head
     int a, b;
     bool has_b;
 };
 
 template <int VEC>
-__device__ __forceinline__ Place<VEC> place_of(const HeadArgs &p, int slot)
+__device__ __forceinline__ Place place_of(const HeadArgs &p, int slot)
 {
-    const int P = (int)p.d.P, D = (int)p.d.D;
-    Place<VEC> at;
-    if (slot < p.rotated && !p.d.interleaved) {
-        at.a = slot * VEC;
-        at.b = P + slot * VEC;
-        at.has_b = true;
-    } else {
-        const int base = slot < p.rotated ? 0 : 2 * P - 2 * VEC * p.rotated;
-        at.a = base + slot * 2 * VEC;
-        at.b = at.a + VEC;
-        at.has_b = at.b < D;
-    }
-    return at;
+    if (slot < p.rotated && !p.d.interleaved) return {slot * VEC, (int)p.d.P + slot * VEC, true};
+    return {slot * 2 * VEC, slot * 2 * VEC + VEC, slot * 2 * VEC + VEC < (int)p.d.D};  // (the rotated slots before it hold 2 P values)
 }
-
-// cosine and sine of wave `pair` of key head j at a position, whole turns dropped
-__device__ __forceinline__ float2 turn_of(const cf_qk_norm &d, const float (&pos)[3], long long j, int pair)
-{
-    const float *w = d.waves + ((d.wave_heads == 1 ? 0 : j) * d.P + pair) * d.C;
-    float whole = 0.f, rest = 0.f;
-#pragma unroll
-    for (int c = 0; c < 3; ++c) {
-        if (c >= d.C) break;
-        const float t = __fmul_rn(pos[c], w[c]), e = __fmaf_rn(pos[c], w[c], -t);
-        whole += t - rintf(t);
-        rest += e - rintf(e);
-    }
-    whole -= rintf(whole);
-    float2 cs;
-    sincospif(2.f * (whole + rest), &cs.y, &cs.x);
-    return cs;
-}
-
-// The slots of one lane: SP of them, `lanes` apart.
-template <class T, int VEC, int SP>
-struct Lane {
-    Place<VEC> at[SP];
-    bool on[SP];
-    float2 cs[SP][VEC];
-
-    __device__ __forceinline__ void init(const HeadArgs &p, int lane)
-    {
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-            const int slot = lane + i * p.lanes;
-            on[i] = slot < p.slots;
-            at[i] = place_of<VEC>(p, on[i] ? slot : 0);
-        }
-    }
-    __device__ __forceinline__ void turn(const HeadArgs &p, int lane, const float (&pos)[3], long long j)
-    {
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-            const int slot = lane + i * p.lanes;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                cs[i][e] = make_float2(1.f, 0.f);
-                if (on[i] && slot < p.rotated) cs[i][e] = turn_of(p.d, pos, j, slot * VEC + e);
-            }
-        }
-    }
-    __device__ __forceinline__ void load(const T *x, float (&a)[SP][VEC], float (&b)[SP][VEC]) const
-    {
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) a[i][e] = b[i][e] = 0.f;
-            if (on[i]) {
-                load_values<T, VEC>(x + at[i].a, a[i]);
-                if (at[i].has_b) load_values<T, VEC>(x + at[i].b, b[i]);
-            }
-        }
-    }
-    __device__ __forceinline__ void store(T *x, const float (&a)[SP][VEC], const float (&b)[SP][VEC]) const
-    {
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-            if (on[i]) {
-                store_values<T, VEC>(x + at[i].a, a[i]);
-                if (at[i].has_b) store_values<T, VEC>(x + at[i].b, b[i]);
-            }
-        }
-    }
-    // the pairs turned by their angles (sign 1) or back (-1)
-    __device__ __forceinline__ void rotate(bool interleaved, float sign, float (&a)[SP][VEC], float (&b)[SP][VEC]) const
-    {
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-            if (interleaved && VEC > 1) {
-#pragma unroll
-                for (int e = 0; e < VEC; e += 2) {
-                    const float2 u = cs[i][e / 2], v = cs[i][VEC / 2 + e / 2];
-                    const float a0 = a[i][e], a1 = a[i][e + 1], b0 = b[i][e], b1 = b[i][e + 1];
-                    a[i][e] = a0 * u.x - sign * a1 * u.y;
-                    a[i][e + 1] = a1 * u.x + sign * a0 * u.y;
-                    b[i][e] = b0 * v.x - sign * b1 * v.y;
-                    b[i][e + 1] = b1 * v.x + sign * b0 * v.y;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float2 u = cs[i][e];
-                    const float x = a[i][e], y = b[i][e];
-                    a[i][e] = x * u.x - sign * y * u.y;
-                    b[i][e] = y * u.x + sign * x * u.y;
-                }
-            }
-        }
-    }
-};
 
 __device__ __forceinline__ float lanes_sum(float v, int lanes)
 {
@@ -160,213 +56,275 @@ __device__ __forceinline__ float lanes_sum(float v, int lanes)
     return v;
 }
 
+// The pairs turned by their angles (sign 1) or back (-1).
 template <int SP, int VEC>
-__device__ __forceinline__ float dot_of(const float (&a)[SP][VEC], const float (&b)[SP][VEC], const float (&c)[SP][VEC], const float (&d)[SP][VEC])
-{
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < SP; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) t += a[i][e] * c[i][e] + b[i][e] * d[i][e];
-    return t;
-}
-
-__device__ __forceinline__ void position_of(const cf_qk_norm &d, long long n, float (&pos)[3])
+__device__ __forceinline__ void rotate(const float2 (&cs)[SP][VEC], bool interleaved, float sign, float (&a)[SP][VEC], float (&b)[SP][VEC])
 {
 #pragma unroll
-    for (int c = 0; c < 3; ++c) pos[c] = d.P > 0 && c < d.C ? d.pos[n * d.C + c] : 0.f;
-}
-
-// Which heads unit u of a token has: key head `key` (or none), query heads [lo, hi); j: the key head whose waves they use.
-struct Unit {
-    long long key, lo, hi, j;
-};
-__device__ __forceinline__ Unit unit_of(const HeadArgs &p, int u)
-{
-    const long long group = p.d.Hk > 0 ? p.d.Hq / p.d.Hk : 1;
-    if (!p.single) return {u, u * group, (u + 1) * group, u};
-    if (u < p.d.Hq) return {-1, u, u + 1, u / group};
-    return {u - p.d.Hq, 0, 0, u - p.d.Hq};
-}
-
-template <class T, int VEC, int SP>
-__global__ void __launch_bounds__(THREADS) qk_norm_fwd_kernel(const HeadArgs p)
-{
-    const int lane = threadIdx.x & (p.lanes - 1), per_block = THREADS / p.lanes;
-    const long long item = (long long)blockIdx.x * per_block + threadIdx.x / p.lanes, items = p.d.N * p.units;
-    // (lanes of a warp beyond the last item go along for the shuffles, with the last one's values, and store nothing)
-    const bool live = item < items;
-    const long long at = live ? item : items - 1, n = at / p.units;
-    const Unit unit = unit_of(p, (int)(at % p.units));
-    Lane<T, VEC, SP> me;
-    me.init(p, lane);
-    float pos[3];
-    position_of(p.d, n, pos);
-    me.turn(p, lane, pos, unit.j);
-    const float inv_d = 1.f / (float)p.d.D, eps = (float)p.d.eps;
-    auto head = [&](const T *x, const T *w, T *to) {
-        float a[SP][VEC], b[SP][VEC];
-        me.load(x, a, b);
-        const float r = rsqrtf(lanes_sum(dot_of(a, b, a, b), p.lanes) * inv_d + eps);
-        if (w != nullptr) {
-            float wa[SP][VEC], wb[SP][VEC];
-            me.load(w, wa, wb);
+    for (int i = 0; i < SP; ++i) {
+        if (interleaved && VEC > 1) {
 #pragma unroll
-            for (int i = 0; i < SP; ++i)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) { a[i][e] *= r * wa[i][e]; b[i][e] *= r * wb[i][e]; }
+            for (int e = 0; e < VEC; e += 2) {
+                const float2 u = cs[i][e / 2], v = cs[i][VEC / 2 + e / 2];
+                const float us = sign * u.y, vs = sign * v.y;
+                const float a0 = a[i][e], a1 = a[i][e + 1], b0 = b[i][e], b1 = b[i][e + 1];
+                a[i][e] = a0 * u.x - a1 * us;
+                a[i][e + 1] = a1 * u.x + a0 * us;
+                b[i][e] = b0 * v.x - b1 * vs;
+                b[i][e + 1] = b1 * v.x + b0 * vs;
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < SP; ++i)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) { a[i][e] *= r; b[i][e] *= r; }
+            for (int e = 0; e < VEC; ++e) {
+                const float c = cs[i][e].x, s = sign * cs[i][e].y, x = a[i][e], y = b[i][e];
+                a[i][e] = x * c - y * s;
+                b[i][e] = y * c + x * s;
+            }
         }
-        me.rotate(p.d.interleaved, 1.f, a, b);
-        if (live) me.store(to, a, b);
-    };
-    const T *wq = static_cast<const T *>(p.d.wq), *wk = static_cast<const T *>(p.d.wk);
-    if (unit.key >= 0)
-        head(static_cast<const T *>(p.d.k) + n * p.d.k_row + unit.key * p.d.k_head, wk == nullptr ? wk : wk + unit.key * p.d.wk_head,
-             static_cast<T *>(p.k_out) + (n * p.d.Hk + unit.key) * p.d.D);
-    for (long long h = unit.lo; h < unit.hi; ++h)
-        head(static_cast<const T *>(p.d.q) + n * p.d.q_row + h * p.d.q_head, wq == nullptr ? wq : wq + h * p.d.wq_head,
-             static_cast<T *>(p.q_out) + (n * p.d.Hq + h) * p.d.D);
+    }
 }
 
-// A lane keeps the sums of its entries' weight gradients for queries and for keys: every unit of a lane's walk is the same one,
-// which has one query head, or weights that its query heads share.
-template <class T, int VEC, int SP>
-__global__ void __launch_bounds__(THREADS) qk_norm_bwd_kernel(const HeadArgs p)
+// Forward and backward: groups of lanes walk the rows, each with one unit of every row's heads.
+template <class T, int VEC, int SP, bool BWD>
+__global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
 {
+    using R = Raw<T, VEC>;
     extern __shared__ float shared[];
-    const int lane = threadIdx.x & (p.lanes - 1), per_block = THREADS / p.lanes;
+    const int lane = threadIdx.x & (p.lanes - 1), per_block = THREADS / p.lanes, D = (int)p.d.D, C = (int)p.d.C;
     const long long group = (long long)blockIdx.x * per_block + threadIdx.x / p.lanes, walk = (long long)gridDim.x * per_block / p.units;
     const bool walks = group < walk * p.units;  // (the last few of a grid that is no multiple of the units have none)
-    const int u = (int)(group % p.units);
-    const Unit unit = unit_of(p, u);
-    Lane<T, VEC, SP> me;
-    me.init(p, lane);
-    const float inv_d = 1.f / (float)p.d.D, eps = (float)p.d.eps;
-    float sum_q[2][SP][VEC], sum_k[2][SP][VEC];
+    const int u = (int)(group % p.units), shared_by = (int)(p.d.Hq / p.d.Hk);
+    // heads of the unit: key head j, then its query heads; or one head alone
+    const bool key_alone = p.single && u >= p.d.Hq;
+    const int j = !p.single ? u : key_alone ? u - (int)p.d.Hq : u / shared_by;
+    const int heads = p.single ? 1 : 1 + shared_by;
+
+    bool on[SP], on_b[SP];
+    Place at[SP];
+    float waves[SP][VEC][3];
+    R wq_raw[SP][2], wk_raw[SP][2];  // (single: the head's in wq_raw)
+    const bool weighted_q = p.d.wq != nullptr, weighted_k = p.d.wk != nullptr;
+    const T *wq = static_cast<const T *>(key_alone ? p.d.wk : p.d.wq), *wk = static_cast<const T *>(p.d.wk);
+    if (key_alone) wq = wq == nullptr ? nullptr : wq + j * p.d.wk_head;
+    else if (wq != nullptr) wq += (p.single ? u : (long long)j * shared_by) * p.d.wq_head;
+    if (wk != nullptr) wk += j * p.d.wk_head;
 #pragma unroll
-    for (int i = 0; i < SP; ++i)
+    for (int i = 0; i < SP; ++i) {
+        const int slot = lane + i * p.lanes;
+        on[i] = slot < p.slots;
+        at[i] = place_of<VEC>(p, on[i] ? slot : 0);
+        on_b[i] = on[i] && at[i].has_b;
+        const bool turns = on[i] && slot < p.rotated;
+        const float *w = p.d.waves + ((p.d.wave_heads == 1 ? 0 : (long long)j) * p.d.P + (long long)slot * VEC) * C;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) sum_q[0][i][e] = sum_q[1][i][e] = sum_k[0][i][e] = sum_k[1][i][e] = 0.f;
-    auto head = [&](const T *x, const T *w, const T *gout, T *to, bool live, float (&sum)[2][SP][VEC]) {
-        float a[SP][VEC], b[SP][VEC], ga[SP][VEC], gb[SP][VEC];
-        me.load(x, a, b);
-        me.load(gout, ga, gb);
-        me.rotate(p.d.interleaved, -1.f, ga, gb);
-        const float r = rsqrtf(lanes_sum(dot_of(a, b, a, b), p.lanes) * inv_d + eps);
-        if (w != nullptr) {
-            float wa[SP][VEC], wb[SP][VEC];
-            me.load(w, wa, wb);
-            const float rl = live ? r : 0.f;
+        for (int e = 0; e < VEC; ++e)
 #pragma unroll
-            for (int i = 0; i < SP; ++i)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (live) {  // (a value that is no number belongs to its own row's sums alone)
-                        sum[0][i][e] += ga[i][e] * (a[i][e] * rl);
-                        sum[1][i][e] += gb[i][e] * (b[i][e] * rl);
-                    }
-                    ga[i][e] *= wa[i][e];
-                    gb[i][e] *= wb[i][e];
-                }
-        }
-        const float m = lanes_sum(dot_of(a, b, ga, gb), p.lanes) * inv_d * r * r;
+            for (int c = 0; c < 3; ++c) waves[i][e][c] = turns && c < C ? w[e * C + c] : 0.f;
+        wq_raw[i][0] = wq_raw[i][1] = wk_raw[i][0] = wk_raw[i][1] = R{};
+        if (wq != nullptr && on[i]) wq_raw[i][0] = load_raw<T, VEC>(wq + at[i].a);
+        if (wq != nullptr && on_b[i]) wq_raw[i][1] = load_raw<T, VEC>(wq + at[i].b);
+        if (wk != nullptr && on[i]) wk_raw[i][0] = load_raw<T, VEC>(wk + at[i].a);
+        if (wk != nullptr && on_b[i]) wk_raw[i][1] = load_raw<T, VEC>(wk + at[i].b);
+    }
+    const float inv_d = 1.f / (float)D, eps = (float)p.d.eps;
+    float sum_q[BWD ? SP : 1][2][VEC], sum_k[BWD ? SP : 1][2][VEC];
+    if constexpr (BWD) {
 #pragma unroll
         for (int i = 0; i < SP; ++i)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                a[i][e] = r * (ga[i][e] - a[i][e] * m);
-                b[i][e] = r * (gb[i][e] - b[i][e] * m);
-            }
-        if (live) me.store(to, a, b);
-    };
-    const T *wq = static_cast<const T *>(p.d.wq), *wk = static_cast<const T *>(p.d.wk);
+            for (int e = 0; e < VEC; ++e) sum_q[i][0][e] = sum_q[i][1][e] = sum_k[i][0][e] = sum_k[i][1][e] = 0.f;
+    }
     // (all lanes of a warp make the same number of steps: those without a row repeat the last one and keep nothing)
-    const long long steps = walk > 0 ? (p.d.N + walk - 1) / walk : 0;
+    const long long row0 = walks ? group / p.units : p.d.N, steps = walk > 0 ? (p.d.N + walk - 1) / walk : 0;
+    auto row_of = [&](long long step) { return min(row0 + step * walk, (long long)p.d.N - 1); };
+    struct Head {
+        bool key;
+        long long h;
+    };
+    auto head_of = [&](int i) { return p.single ? Head{key_alone, key_alone ? j : u} : Head{i == 0, i == 0 ? j : (long long)j * shared_by + i - 1}; };
+    R xa[SP], xb[SP], ga[BWD ? SP : 1], gb[BWD ? SP : 1];
+    float pos[3];
+    auto fetch = [&](long long step, int i) {
+        const long long n = row_of(step);
+        const Head hd = head_of(i);
+        const T *x = hd.key ? static_cast<const T *>(p.d.k) + n * p.d.k_row + hd.h * p.d.k_head : static_cast<const T *>(p.d.q) + n * p.d.q_row + hd.h * p.d.q_head;
+        const T *g = nullptr;
+        if constexpr (BWD) g = static_cast<const T *>(hd.key ? p.gk_out : p.gq_out) + (n * (hd.key ? p.d.Hk : p.d.Hq) + hd.h) * D;
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+            xa[s] = xb[s] = R{};
+            if (on[s]) xa[s] = load_raw<T, VEC>(x + at[s].a);
+            if (on_b[s]) xb[s] = load_raw<T, VEC>(x + at[s].b);
+            if constexpr (BWD) {
+                ga[s] = gb[s] = R{};
+                if (on[s]) ga[s] = load_raw<T, VEC>(g + at[s].a);
+                if (on_b[s]) gb[s] = load_raw<T, VEC>(g + at[s].b);
+            }
+        }
+        if (i == 0) {
+#pragma unroll
+            for (int c = 0; c < 3; ++c) pos[c] = p.d.P > 0 && c < C ? p.d.pos[n * C + c] : 0.f;
+        }
+    };
+    if (steps > 0) fetch(0, 0);
+    float2 cs[SP][VEC];
     for (long long step = 0; step < steps; ++step) {
-        const long long row = group / p.units + step * walk;
-        const bool live = walks && row < p.d.N;
-        const long long n = live ? row : p.d.N - 1;
-        float pos[3];
-        position_of(p.d, n, pos);
-        me.turn(p, lane, pos, unit.j);
-        auto query = [&](long long h) {
-            head(static_cast<const T *>(p.d.q) + n * p.d.q_row + h * p.d.q_head, wq == nullptr ? wq : wq + h * p.d.wq_head,
-                 static_cast<const T *>(p.gq_out) + (n * p.d.Hq + h) * p.d.D, static_cast<T *>(p.q_out) + (n * p.d.Hq + h) * p.d.D, live, sum_q);
-        };
-        if (!p.single) {
-            head(static_cast<const T *>(p.d.k) + n * p.d.k_row + unit.j * p.d.k_head, wk == nullptr ? wk : wk + unit.j * p.d.wk_head,
-                 static_cast<const T *>(p.gk_out) + (n * p.d.Hk + unit.j) * p.d.D, static_cast<T *>(p.k_out) + (n * p.d.Hk + unit.j) * p.d.D, live, sum_k);
-            for (long long h = unit.lo; h < unit.hi; ++h) query(h);
-        } else {  // (the heads of a warp's lanes differ: one call for either kind, as they shuffle together)
-            const bool is_key = unit.key >= 0;
-            const long long h = is_key ? unit.key : unit.lo, H = is_key ? p.d.Hk : p.d.Hq;
-            const T *x = static_cast<const T *>(is_key ? p.d.k : p.d.q) + n * (is_key ? p.d.k_row : p.d.q_row) + h * (is_key ? p.d.k_head : p.d.q_head);
-            const T *w = is_key ? (wk == nullptr ? wk : wk + h * p.d.wk_head) : wq + h * p.d.wq_head;
-            const long long at = (n * H + h) * p.d.D;
-            head(x, w, static_cast<const T *>(is_key ? p.gk_out : p.gq_out) + at, static_cast<T *>(is_key ? p.k_out : p.q_out) + at, live, sum_q);
+        const bool live = row0 + step * walk < p.d.N;
+        const long long n = row_of(step);
+        // the angles of the row: exact products, whole turns dropped
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+            if (lane + s * p.lanes >= p.rotated) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) cs[s][e] = make_float2(1.f, 0.f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    float whole = 0.f, rest = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 3; ++c) {
+                        if (c >= C) break;
+                        const float t = __fmul_rn(pos[c], waves[s][e][c]), r = __fmaf_rn(pos[c], waves[s][e][c], -t);
+                        whole += t - rintf(t);
+                        rest += r - rintf(r);
+                    }
+                    whole -= rintf(whole);
+                    sincospif(2.f * (whole + rest), &cs[s][e].y, &cs[s][e].x);
+                }
+            }
+        }
+        for (int i = 0; i < heads; ++i) {
+            const Head hd = head_of(i);
+            float a[SP][VEC], b[SP][VEC], fa[BWD ? SP : 1][VEC], fb[BWD ? SP : 1][VEC];
+            float square = 0.f;
+#pragma unroll
+            for (int s = 0; s < SP; ++s) {
+                expand<T, VEC>(xa[s], a[s]);
+                expand<T, VEC>(xb[s], b[s]);
+                if constexpr (BWD) {
+                    expand<T, VEC>(ga[s], fa[s]);
+                    expand<T, VEC>(gb[s], fb[s]);
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) square += a[s][e] * a[s][e] + b[s][e] * b[s][e];
+            }
+            // the next head's values, then the next row's
+            const bool last = i + 1 == heads;
+            if (!last || step + 1 < steps) fetch(last ? step + 1 : step, last ? 0 : i + 1);
+            const float r = rsqrtf(lanes_sum(square, p.lanes) * inv_d + eps);
+            const bool of_k = !p.single && i == 0, weighted = key_alone || of_k ? weighted_k : weighted_q;
+            T *to = static_cast<T *>(hd.key ? p.k_out : p.q_out) + (n * (hd.key ? p.d.Hk : p.d.Hq) + hd.h) * D;
+            if constexpr (!BWD) {
+#pragma unroll
+                for (int s = 0; s < SP; ++s) {
+                    float wa[VEC], wb[VEC];
+                    expand<T, VEC>(of_k ? wk_raw[s][0] : wq_raw[s][0], wa);
+                    expand<T, VEC>(of_k ? wk_raw[s][1] : wq_raw[s][1], wb);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        a[s][e] *= r;
+                        b[s][e] *= r;
+                        if (weighted) { a[s][e] *= wa[e]; b[s][e] *= wb[e]; }
+                    }
+                }
+                rotate(cs, p.d.interleaved, 1.f, a, b);
+            } else {
+                rotate(cs, p.d.interleaved, -1.f, fa, fb);
+                float dot = 0.f;
+#pragma unroll
+                for (int s = 0; s < SP; ++s) {
+                    float wa[VEC], wb[VEC];
+                    expand<T, VEC>(of_k ? wk_raw[s][0] : wq_raw[s][0], wa);
+                    expand<T, VEC>(of_k ? wk_raw[s][1] : wq_raw[s][1], wb);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        a[s][e] *= r;  // x r from here on
+                        b[s][e] *= r;
+                        if (weighted) {
+                            if (live) {  // (a value that is no number belongs to its own row's sums alone)
+                                const float ta = fa[s][e] * a[s][e], tb = fb[s][e] * b[s][e];
+                                if (of_k) { sum_k[s][0][e] += ta; sum_k[s][1][e] += tb; }
+                                else { sum_q[s][0][e] += ta; sum_q[s][1][e] += tb; }
+                            }
+                            fa[s][e] *= wa[e];
+                            fb[s][e] *= wb[e];
+                        }
+                        dot += a[s][e] * fa[s][e] + b[s][e] * fb[s][e];
+                    }
+                }
+                const float m = lanes_sum(dot, p.lanes) * inv_d;
+#pragma unroll
+                for (int s = 0; s < SP; ++s)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        a[s][e] = r * (fa[s][e] - a[s][e] * m);
+                        b[s][e] = r * (fb[s][e] - b[s][e] * m);
+                    }
+            }
+            if (live) {
+#pragma unroll
+                for (int s = 0; s < SP; ++s) {
+                    if (on[s]) store_values<T, VEC>(to + at[s].a, a[s]);
+                    if (on_b[s]) store_values<T, VEC>(to + at[s].b, b[s]);
+                }
+            }
         }
     }
-    if (p.partial == nullptr) return;
-    // (block, query or key, unit, entry)
-    const int D = (int)p.d.D;
-    for (int which = 0; which < (p.single ? 1 : 2); ++which) {  // (single: the unit says which)
-        float(&sum)[2][SP][VEC] = which ? sum_k : sum_q;
-        __syncthreads();
-        float *mine = shared + (size_t)(threadIdx.x / p.lanes) * D;
-#pragma unroll
-        for (int i = 0; i < SP; ++i) {
-            if (!me.on[i]) continue;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                mine[me.at[i].a + e] = sum[0][i][e];
-                if (me.at[i].has_b) mine[me.at[i].b + e] = sum[1][i][e];
-            }
-        }
-        __syncthreads();
-        float *to = p.partial + ((size_t)blockIdx.x * 2 + which) * p.units * D;
+    if constexpr (BWD) {
+        if (p.partial == nullptr) return;
         const int first = (int)(((long long)blockIdx.x * per_block) % p.units);  // the block's first unit
-        for (int at = threadIdx.x; at < p.units * D; at += THREADS) {
-            const int v = at / D, d = at % D;
-            float t = 0.f;
-            for (int g = (v - first + p.units) % p.units; g < per_block; g += p.units) t += shared[(size_t)g * D + d];
-            to[at] = t;
+        for (int which = 0; which < 2; ++which) {  // the queries' weights, the keys'
+            const int begin = which ? p.columns_q : 0, end = which ? p.columns : p.columns_q;
+            if (!(which && p.single)) {  // (single: all sums are in sum_q, and are there already)
+                __syncthreads();
+                float *mine = shared + (size_t)(threadIdx.x / p.lanes) * D;
+#pragma unroll
+                for (int s = 0; s < SP; ++s) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        if (on[s]) mine[at[s].a + e] = which ? sum_k[s][0][e] : sum_q[s][0][e];
+                        if (on_b[s]) mine[at[s].b + e] = which ? sum_k[s][1][e] : sum_q[s][1][e];
+                    }
+                }
+                __syncthreads();
+            }
+            const bool each = end - begin > D;  // one set of sums per head (or there is one head)
+            const int unit0 = p.single && which ? (int)p.d.Hq : 0, units = p.single ? (int)(which ? p.d.Hk : p.d.Hq) : p.units;
+            for (int c = begin + threadIdx.x; c < end; c += THREADS) {
+                const int set = (c - begin) / D, d = (c - begin) % D;
+                float t = 0.f;
+                if (each || units == 1) {
+                    for (int g = (unit0 + set - first + p.units) % p.units; g < per_block; g += p.units) t += shared[(size_t)g * D + d];
+                } else {
+                    for (int g = 0; g < per_block; ++g) {
+                        const int v = (first + g) % p.units - unit0;
+                        if (v >= 0 && v < units) t += shared[(size_t)g * D + d];
+                    }
+                }
+                p.partial[(size_t)blockIdx.x * p.columns + c] = t;
+            }
         }
     }
 }
 
-// The blocks' sums, in their order: thread (x, y) column x of a unit's entry, the y-th share of the blocks.
+// The blocks' sums, in a fixed order: 32 columns, a block's 32 warps a share of the blocks each.
 template <class T>
-__global__ void __launch_bounds__(256) qk_weight_sum_kernel(const HeadArgs p, int blocks, T *gwq, T *gwk)
+__global__ void __launch_bounds__(1024) qk_weight_sum_kernel(const float *partial, int blocks, int columns, int columns_q, T *gwq, T *gwk)
 {
-    __shared__ float part[8][32];
-    const int which = blockIdx.y, D = (int)p.d.D, lane = threadIdx.x & 31, share = threadIdx.x >> 5;
-    T *to = which ? gwk : gwq;
-    if (to == nullptr) return;
-    const long long heads = which ? p.d.Hk : p.d.Hq;
-    const bool each = (which ? p.d.wk_head : p.d.wq_head) != 0;
-    // outputs: (heads, D), or (D) summed over the units
-    const long long outs = each ? heads * D : D, at = (long long)blockIdx.x * 32 + lane;
+    __shared__ float part[32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float t = 0.f;
-    if (at < outs) {
-        const int d = (int)(at % D);
-        const long long h = at / D;
-        // the units that hold it: of shared weights all; else the one of this head
-        const long long u0 = (p.single && which ? p.d.Hq : 0) + (each ? h : 0), u1 = each ? u0 + 1 : p.units;
-        for (int b = share; b < blocks; b += 8)
-            for (long long u = u0; u < u1; ++u) t += p.partial[(((size_t)b * 2 + (p.single ? 0 : which)) * p.units + u) * D + d];
+    if (c < columns) {
+#pragma unroll 8
+        for (int b = warp; b < blocks; b += 32) t += partial[(size_t)b * columns + c];
     }
-    part[share][lane] = t;
+    part[warp][lane] = t;
     __syncthreads();
-    if (share == 0 && at < outs) {
+    if (warp > 0 || c >= columns) return;
 #pragma unroll
-        for (int s = 1; s < 8; ++s) t += part[s][lane];
-        to[at] = from_float<T>(t);
-    }
+    for (int w = 1; w < 32; ++w) t += part[w][lane];
+    T *to = c < columns_q ? gwq : gwk;
+    if (to != nullptr) to[c < columns_q ? c : c - columns_q] = from_float<T>(t);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
@@ -405,74 +363,77 @@ bool fits(const HeadArgs &a, int vec, bool backward)
     return !backward || (aligned_to(a.gq_out, bytes) && aligned_to(a.gk_out, bytes));
 }
 
-constexpr int BWD_BLOCKS_PER_SM = 6;
+constexpr int MAX_BLOCKS_PER_SM = 8;  // (2,048 threads)
 
-long long bwd_blocks(long long items, int per_block)  // (no more groups than there are items)
+// Blocks: `at_once` per SM walk the rows; no more groups than there are items, but every unit is walked.
+long long blocks_of(long long items, int units, int per_block, int at_once)
 {
-    const long long cap = (long long)sm_count() * BWD_BLOCKS_PER_SM, need = (items + per_block - 1) / per_block;
-    return need < cap ? need : cap;
+    const long long cap = (long long)sm_count() * at_once, need = (items + per_block - 1) / per_block, least = (units + per_block - 1) / per_block;
+    const long long blocks = need < cap ? need : cap;
+    return blocks > least ? blocks : least;
 }
 
-int units_of(const cf_qk_norm &d, bool backward, int &single)
+int units_of(const cf_qk_norm &d, int &single)
 {
-    // per-head query weights with several query heads to a key head: one head per unit, so that a lane has one set of sums
-    single = backward && d.Hq != d.Hk && d.wq != nullptr && d.wq_head != 0;
+    // query weights of each head, several query heads to a key head: one head per unit, so that a lane has one set of weights
+    single = d.Hq != d.Hk && d.wq != nullptr && d.wq_head != 0;
     return (int)(single ? d.Hq + d.Hk : d.Hk);
 }
 
-template <class T, int VEC, int SP>
-int launch_sp(const HeadArgs &a, bool backward, void *gwq, void *gwk, cudaStream_t s)
+template <class T, int VEC, int SP, bool BWD>
+int launch_sp(const HeadArgs &a, void *gwq, void *gwk, cudaStream_t s)
 {
+    static thread_local int resident[64] = {};
     const int per_block = THREADS / a.lanes;
-    const long long items = a.d.N * a.units;
-    if (!backward) {
-        qk_norm_fwd_kernel<T, VEC, SP><<<(unsigned)((items + per_block - 1) / per_block), THREADS, 0, s>>>(a);
-        return launch_status("qk_norm_fwd_kernel");
+    const size_t smem = BWD && a.partial ? (size_t)per_block * a.d.D * sizeof(float) : 0;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int &at_once = resident[dev & 63];
+    if (at_once == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, qk_norm_kernel<T, VEC, SP, BWD>, THREADS, 16384) != cudaSuccess || at_once < 1) {
+            cudaGetLastError();
+            at_once = 1;
+        }
+        if (at_once > MAX_BLOCKS_PER_SM) at_once = MAX_BLOCKS_PER_SM;
     }
-    long long blocks = bwd_blocks(items, per_block);
-    if (blocks * per_block < a.units) blocks = (a.units + per_block - 1) / per_block;  // (every unit is walked)
-    const size_t smem = a.partial ? (size_t)per_block * a.d.D * sizeof(float) : 0;
-    qk_norm_bwd_kernel<T, VEC, SP><<<(unsigned)blocks, THREADS, smem, s>>>(a);
-    if (a.partial != nullptr) {
-        const long long outs = (a.d.wq_head || a.d.wk_head ? a.d.Hq : 1) * a.d.D;
-        qk_weight_sum_kernel<T><<<dim3((unsigned)((outs + 31) / 32), 2), 256, 0, s>>>(a, (int)blocks, static_cast<T *>(gwq), static_cast<T *>(gwk));
-    }
-    return launch_status("qk_norm_bwd_kernel");
+    const long long blocks = blocks_of(a.d.N * a.units, a.units, per_block, at_once);
+    qk_norm_kernel<T, VEC, SP, BWD><<<(unsigned)blocks, THREADS, smem, s>>>(a);
+    if (BWD && a.partial != nullptr)
+        qk_weight_sum_kernel<T><<<(a.columns + 31) / 32, 1024, 0, s>>>(a.partial, (int)blocks, a.columns, a.columns_q, static_cast<T *>(gwq), static_cast<T *>(gwk));
+    return launch_status("qk_norm_kernel");
 }
 
-template <class T, int VEC>
-int launch_vec(HeadArgs a, bool backward, void *gwq, void *gwk, cudaStream_t s)
+template <class T, int VEC, bool BWD>
+int launch_vec(HeadArgs a, void *gwq, void *gwk, cudaStream_t s)
 {
     a.rotated = (int)(a.d.P / VEC);
     a.slots = a.rotated + (int)((a.d.D - 2 * a.d.P + 2 * VEC - 1) / (2 * VEC));
     a.lanes = 1;
     while (a.lanes < 32 && a.lanes < a.slots) a.lanes *= 2;
     const int sp = (a.slots + a.lanes - 1) / a.lanes;
-    if (sp <= 1) return launch_sp<T, VEC, 1>(a, backward, gwq, gwk, s);
-    if constexpr (VEC <= 4) {  // (heads of up to 512: 32 slots of 16 values, 64 of 8, 256 of 2)
-        if (sp <= 2) return launch_sp<T, VEC, 2>(a, backward, gwq, gwk, s);
-    }
-    if constexpr (VEC == 1) return launch_sp<T, VEC, 8>(a, backward, gwq, gwk, s);
+    if (sp <= 1) return launch_sp<T, VEC, 1, BWD>(a, gwq, gwk, s);
+    if (sp <= 2) return launch_sp<T, VEC, 2, BWD>(a, gwq, gwk, s);  // (heads of up to 512: 64 slots of 8 values, 256 of 2)
+    if constexpr (VEC == 1) return launch_sp<T, VEC, 8, BWD>(a, gwq, gwk, s);
     return fail(CF_ERR_RANGE, "cf_qk_norm: heads of %lld", (long long)a.d.D);
 }
 
-template <class T>
-int launch(const HeadArgs &a, bool backward, void *gwq, void *gwk, cudaStream_t s)
+template <class T, bool BWD>
+int launch(const HeadArgs &a, void *gwq, void *gwk, cudaStream_t s)
 {
-    if constexpr (sizeof(T) == 2) {
-        if (fits(a, 8, backward)) return launch_vec<T, 8>(a, backward, gwq, gwk, s);
-    }
-    if (fits(a, 4, backward)) return launch_vec<T, 4>(a, backward, gwq, gwk, s);
-    return launch_vec<T, 1>(a, backward, gwq, gwk, s);
+    if (fits(a, 4, BWD)) return launch_vec<T, 4, BWD>(a, gwq, gwk, s);
+    return launch_vec<T, 1, BWD>(a, gwq, gwk, s);
 }
 
-int launch_typed(HeadArgs &a, bool backward, void *gwq, void *gwk, void *stream)
+template <bool BWD>
+int launch_typed(HeadArgs &a, void *gwq, void *gwk, void *stream)
 {
-    a.units = units_of(a.d, backward, a.single);
+    a.units = units_of(a.d, a.single);
+    a.columns_q = a.d.wq ? (int)((a.d.wq_head ? a.d.Hq : 1) * a.d.D) : 0;
+    a.columns = a.columns_q + (a.d.wk ? (int)((a.d.wk_head ? a.d.Hk : 1) * a.d.D) : 0);
     cudaStream_t s = as_stream(stream);
-    if (a.d.type == CF_FLOAT32) return launch<float>(a, backward, gwq, gwk, s);
-    if (a.d.type == CF_BFLOAT16) return launch<__nv_bfloat16>(a, backward, gwq, gwk, s);
-    return launch<__half>(a, backward, gwq, gwk, s);
+    if (a.d.type == CF_FLOAT32) return launch<float, BWD>(a, gwq, gwk, s);
+    if (a.d.type == CF_BFLOAT16) return launch<__nv_bfloat16, BWD>(a, gwq, gwk, s);
+    return launch<__half, BWD>(a, gwq, gwk, s);
 }
 
 }  // namespace
@@ -492,19 +453,18 @@ int cf_qk_norm_fwd(const cf_qk_norm *args, void *q_out, void *k_out, void *strea
     a.d = *args;
     a.q_out = q_out;
     a.k_out = k_out;
-    return launch_typed(a, false, nullptr, nullptr, stream);
+    return launch_typed<false>(a, nullptr, nullptr, stream);
 }
 
 int64_t cf_qk_norm_bwd_workspace_bytes(const cf_qk_norm *args)
 {
     if (check_args("cf_qk_norm_bwd_workspace_bytes", args) != CF_OK) return 0;
     int single = 0;
-    const int units = units_of(*args, true, single);
-    // blocks of at least eight heads' lanes each; the most that a launch of any vector width has
-    long long blocks = bwd_blocks(args->N * units, THREADS / 32);
-    const long long least = (units + THREADS / 32 - 1) / (THREADS / 32);
-    if (blocks < least) blocks = least;
-    return (int64_t)((size_t)blocks * 2 * units * args->D * sizeof(float));
+    const int units = units_of(*args, single);
+    // blocks of eight groups at least, as many as an SM holds at most: no launch of the call has more
+    const long long blocks = blocks_of(args->N * units, units, THREADS / 32, MAX_BLOCKS_PER_SM);
+    const long long columns = (args->wq ? (args->wq_head ? args->Hq : 1) : 0) + (args->wk ? (args->wk_head ? args->Hk : 1) : 0);
+    return (int64_t)((size_t)blocks * columns * args->D * sizeof(float));
 }
 
 int cf_qk_norm_bwd(const cf_qk_norm *args, const void *gq_out, const void *gk_out, void *gq, void *gk, void *gwq, void *gwk, void *workspace, void *stream)
@@ -528,7 +488,7 @@ int cf_qk_norm_bwd(const cf_qk_norm *args, const void *gq_out, const void *gk_ou
     a.q_out = gq;
     a.k_out = gk;
     a.partial = gwq || gwk ? static_cast<float *>(workspace) : nullptr;
-    return launch_typed(a, true, gwq, gwk, stream);
+    return launch_typed<true>(a, gwq, gwk, stream);
 }
 
 }  // extern "C"

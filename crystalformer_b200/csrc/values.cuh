@@ -84,6 +84,31 @@ __device__ __forceinline__ void store_values(T *p, const float (&v)[VEC])
     }
 }
 
+// ... held as they lie in memory, to be converted when they are needed
+template <int BYTES> struct RawBytes;
+template <> struct RawBytes<16> { using type = uint4; };
+template <> struct RawBytes<8> { using type = uint2; };
+template <> struct RawBytes<4> { using type = uint32_t; };
+template <> struct RawBytes<2> { using type = uint16_t; };
+template <class T, int VEC> using Raw = typename RawBytes<VEC * sizeof(T)>::type;
+template <class T, int VEC> __device__ __forceinline__ Raw<T, VEC> load_raw(const T *p) { return *reinterpret_cast<const Raw<T, VEC> *>(p); }
+template <class T, int VEC>
+__device__ __forceinline__ void expand(const Raw<T, VEC> &raw, float (&v)[VEC])
+{
+    if constexpr (VEC == 1 || sizeof(T) == 4) {
+        const T *t = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = to_float(t[i]);
+    } else {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(&raw);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            const float2 f = unpack_two<T>(w[i]);
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+    }
+}
+
 // 32 neighbouring bytes, aligned to that, in one store
 __device__ __forceinline__ void store_32(void *p, const uint32_t (&w)[8])
 {
