@@ -8,11 +8,11 @@
 // Bound by memory (2 + 2 bytes or 4 + 4 a value forward), as long as the sines do not dominate: an angle is computed once per key
 // head and used for that key head and the query heads that share it.  A head is held by the fewest lanes (a power of two) that
 // take it in slots of 2 VEC values - a pair of vectors whose entries are partners - so that sums of squares are a few shuffles and
-// nothing is exchanged for the rotation.  A group of lanes walks the rows with the same heads of each: its weights and waves stay in
-// registers, and the next head's values are on their way while one is computed (without that, and with 16-byte vectors' twice as
+// nothing is exchanged for the rotation.  A group of lanes walks the rows with the same heads of each; the next head's values are
+// on their way while one is computed (without that, and with 16-byte vectors' twice as
 // many registers, the backward of 16,384 rows of 32 + 8 heads of 128 took 353 us).  Waves count cycles per unit of position: the
 // products are exact (a rounded product and its fused remainder), whole turns are dropped before the parts are added, and an angle
-// is off by 2^-24 turns however far the position; whole-numbered waves on fractional coordinates thus do not see lattice
+// is off by 2^-24 turns out to 2^24 turns of an axis; whole-numbered waves on fractional coordinates thus do not see lattice
 // translations at all.
 //
 // The weights' gradients are sums over all rows: each lane keeps its entries' in registers, a block adds its lanes' in a fixed order,
@@ -84,9 +84,54 @@ __device__ __forceinline__ void rotate(const float2 (&cs)[SP][VEC], bool interle
     }
 }
 
+// Cosines and sines of a lane's pairs at a row's position: exact products, whole turns dropped.  The waves come from L1 (12 registers
+// less than keeping them, and a third block on the SM).
+template <class T, int VEC, int SP, int C>
+__device__ __forceinline__ void row_angles(const HeadArgs &p, const float *waves, int lane, const float (&pos)[3], float2 (&cs)[SP][VEC])
+{
+#pragma unroll
+    for (int s = 0; s < SP; ++s) {
+        const int slot = lane + s * p.lanes;
+        if (slot >= p.rotated) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) cs[s][e] = make_float2(1.f, 0.f);
+            continue;
+        }
+        float w[VEC * C];
+        const float *at = waves + (long long)slot * VEC * C;
+        if constexpr (VEC == 1) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) w[c] = __ldg(at + c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC * C / 4; ++i) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(at) + i);
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            float whole = 0.f, rest = 0.f;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const float t = __fmul_rn(pos[c], w[e * C + c]);
+                rest += __fmaf_rn(pos[c], w[e * C + c], -t);
+                whole += t - rintf(t);
+            }
+            if constexpr (sizeof(T) == 2) {  // (the sine of the special functions: 2^-21 off, a thousandth of a 16-bit half step)
+                whole += rest;
+                whole -= rintf(whole);
+                __sincosf(6.283185307179586f * whole, &cs[s][e].y, &cs[s][e].x);
+            } else {
+                sincospif(2.f * (whole + rest), &cs[s][e].y, &cs[s][e].x);
+            }
+        }
+    }
+}
+
 // Forward and backward: groups of lanes walk the rows, each with one unit of every row's heads.
 template <class T, int VEC, int SP, bool BWD>
-__global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
+__global__ void __launch_bounds__(THREADS, SP > 1 ? 1 : BWD || VEC == 8 ? 2 : 3) qk_norm_kernel(const HeadArgs p)
 {
     using R = Raw<T, VEC>;
     extern __shared__ float shared[];
@@ -101,8 +146,8 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
 
     bool on[SP], on_b[SP];
     Place at[SP];
-    float waves[SP][VEC][3];
-    R wq_raw[SP][2], wk_raw[SP][2];  // (single: the head's in wq_raw)
+    constexpr bool KEEP = BWD || VEC == 8;  // the weights in registers; else they come from L1 head by head, for a third block on the SM
+    R wq_raw[KEEP ? SP : 1][2], wk_raw[KEEP ? SP : 1][2];  // (single: the head's in wq_raw)
     const bool weighted_q = p.d.wq != nullptr, weighted_k = p.d.wk != nullptr;
     const T *wq = static_cast<const T *>(key_alone ? p.d.wk : p.d.wq), *wk = static_cast<const T *>(p.d.wk);
     if (key_alone) wq = wq == nullptr ? nullptr : wq + j * p.d.wk_head;
@@ -114,17 +159,13 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
         on[i] = slot < p.slots;
         at[i] = place_of<VEC>(p, on[i] ? slot : 0);
         on_b[i] = on[i] && at[i].has_b;
-        const bool turns = on[i] && slot < p.rotated;
-        const float *w = p.d.waves + ((p.d.wave_heads == 1 ? 0 : (long long)j) * p.d.P + (long long)slot * VEC) * C;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-#pragma unroll
-            for (int c = 0; c < 3; ++c) waves[i][e][c] = turns && c < C ? w[e * C + c] : 0.f;
-        wq_raw[i][0] = wq_raw[i][1] = wk_raw[i][0] = wk_raw[i][1] = R{};
-        if (wq != nullptr && on[i]) wq_raw[i][0] = load_raw<T, VEC>(wq + at[i].a);
-        if (wq != nullptr && on_b[i]) wq_raw[i][1] = load_raw<T, VEC>(wq + at[i].b);
-        if (wk != nullptr && on[i]) wk_raw[i][0] = load_raw<T, VEC>(wk + at[i].a);
-        if (wk != nullptr && on_b[i]) wk_raw[i][1] = load_raw<T, VEC>(wk + at[i].b);
+        if constexpr (KEEP) {
+            wq_raw[i][0] = wq_raw[i][1] = wk_raw[i][0] = wk_raw[i][1] = R{};
+            if (wq != nullptr && on[i]) wq_raw[i][0] = load_raw<T, VEC>(wq + at[i].a);
+            if (wq != nullptr && on_b[i]) wq_raw[i][1] = load_raw<T, VEC>(wq + at[i].b);
+            if (wk != nullptr && on[i]) wk_raw[i][0] = load_raw<T, VEC>(wk + at[i].a);
+            if (wk != nullptr && on_b[i]) wk_raw[i][1] = load_raw<T, VEC>(wk + at[i].b);
+        }
     }
     const float inv_d = 1.f / (float)D, eps = (float)p.d.eps;
     float sum_q[BWD ? SP : 1][2][VEC], sum_k[BWD ? SP : 1][2][VEC];
@@ -135,21 +176,25 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
             for (int e = 0; e < VEC; ++e) sum_q[i][0][e] = sum_q[i][1][e] = sum_k[i][0][e] = sum_k[i][1][e] = 0.f;
     }
     // (all lanes of a warp make the same number of steps: those without a row repeat the last one and keep nothing)
-    const long long row0 = walks ? group / p.units : p.d.N, steps = walk > 0 ? (p.d.N + walk - 1) / walk : 0;
-    auto row_of = [&](long long step) { return min(row0 + step * walk, (long long)p.d.N - 1); };
-    struct Head {
-        bool key;
-        long long h;
-    };
-    auto head_of = [&](int i) { return p.single ? Head{key_alone, key_alone ? j : u} : Head{i == 0, i == 0 ? j : (long long)j * shared_by + i - 1}; };
+    const int N = (int)p.d.N, row0 = walks ? (int)(group / p.units) : N, steps = walk > 0 ? (int)((N + walk - 1) / walk) : 0;
+    auto row_of = [&](int step) { return (int)min(row0 + step * walk, (long long)N - 1); };
+    // the heads' places in a row: key head j, query heads of it (single: the one head, in the queries' place)
+    const int q0 = p.single ? (key_alone ? j : u) : j * shared_by;
+    const T *kx = static_cast<const T *>(p.d.k) + (long long)j * p.d.k_head;
+    const T *qx = key_alone ? kx : static_cast<const T *>(p.d.q) + (long long)q0 * p.d.q_head;
+    const int k_row = (int)p.d.k_row, q_row = key_alone ? k_row : (int)p.d.q_row, q_head = (int)p.d.q_head;
+    const int k_out_row = (int)p.d.Hk * D, q_out_row = key_alone ? k_out_row : (int)p.d.Hq * D;
+    const T *gkx = static_cast<const T *>(p.gk_out) + j * D, *gqx = key_alone ? gkx : static_cast<const T *>(p.gq_out) + q0 * D;
+    T *ky = static_cast<T *>(p.k_out) + j * D, *qy = key_alone ? ky : static_cast<T *>(p.q_out) + q0 * D;
     R xa[SP], xb[SP], ga[BWD ? SP : 1], gb[BWD ? SP : 1];
     float pos[3];
-    auto fetch = [&](long long step, int i) {
-        const long long n = row_of(step);
-        const Head hd = head_of(i);
-        const T *x = hd.key ? static_cast<const T *>(p.d.k) + n * p.d.k_row + hd.h * p.d.k_head : static_cast<const T *>(p.d.q) + n * p.d.q_row + hd.h * p.d.q_head;
+    auto fetch = [&](int step, int i) {
+        const int n = row_of(step);
+        const bool of_k = !p.single && i == 0;
+        const int at_q = p.single ? 0 : i - 1;
+        const T *x = of_k ? kx + (long long)n * k_row : qx + (long long)n * q_row + at_q * q_head;
         const T *g = nullptr;
-        if constexpr (BWD) g = static_cast<const T *>(hd.key ? p.gk_out : p.gq_out) + (n * (hd.key ? p.d.Hk : p.d.Hq) + hd.h) * D;
+        if constexpr (BWD) g = of_k ? gkx + (long long)n * k_out_row : gqx + (long long)n * q_out_row + at_q * D;
 #pragma unroll
         for (int s = 0; s < SP; ++s) {
             xa[s] = xb[s] = R{};
@@ -163,38 +208,19 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
         }
         if (i == 0) {
 #pragma unroll
-            for (int c = 0; c < 3; ++c) pos[c] = p.d.P > 0 && c < C ? p.d.pos[n * C + c] : 0.f;
+            for (int c = 0; c < 3; ++c) pos[c] = p.d.P > 0 && c < C ? p.d.pos[(long long)n * C + c] : 0.f;
         }
     };
     if (steps > 0) fetch(0, 0);
+    const float *wave0 = p.d.waves + (p.d.wave_heads == 1 ? 0 : (long long)j) * p.d.P * C;
     float2 cs[SP][VEC];
-    for (long long step = 0; step < steps; ++step) {
-        const bool live = row0 + step * walk < p.d.N;
-        const long long n = row_of(step);
-        // the angles of the row: exact products, whole turns dropped
-#pragma unroll
-        for (int s = 0; s < SP; ++s) {
-            if (lane + s * p.lanes >= p.rotated) {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) cs[s][e] = make_float2(1.f, 0.f);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    float whole = 0.f, rest = 0.f;
-#pragma unroll
-                    for (int c = 0; c < 3; ++c) {
-                        if (c >= C) break;
-                        const float t = __fmul_rn(pos[c], waves[s][e][c]), r = __fmaf_rn(pos[c], waves[s][e][c], -t);
-                        whole += t - rintf(t);
-                        rest += r - rintf(r);
-                    }
-                    whole -= rintf(whole);
-                    sincospif(2.f * (whole + rest), &cs[s][e].y, &cs[s][e].x);
-                }
-            }
-        }
+    for (int step = 0; step < steps; ++step) {
+        const bool live = row0 + step * walk < N;
+        const int n = row_of(step);
+        if (C == 3) row_angles<T, VEC, SP, 3>(p, wave0, lane, pos, cs);
+        else if (C == 2) row_angles<T, VEC, SP, 2>(p, wave0, lane, pos, cs);
+        else row_angles<T, VEC, SP, 1>(p, wave0, lane, pos, cs);
         for (int i = 0; i < heads; ++i) {
-            const Head hd = head_of(i);
             float a[SP][VEC], b[SP][VEC], fa[BWD ? SP : 1][VEC], fb[BWD ? SP : 1][VEC];
             float square = 0.f;
 #pragma unroll
@@ -211,15 +237,28 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
             // the next head's values, then the next row's
             const bool last = i + 1 == heads;
             if (!last || step + 1 < steps) fetch(last ? step + 1 : step, last ? 0 : i + 1);
-            const float r = rsqrtf(lanes_sum(square, p.lanes) * inv_d + eps);
             const bool of_k = !p.single && i == 0, weighted = key_alone || of_k ? weighted_k : weighted_q;
-            T *to = static_cast<T *>(hd.key ? p.k_out : p.q_out) + (n * (hd.key ? p.d.Hk : p.d.Hq) + hd.h) * D;
+            R wa_raw[SP], wb_raw[SP];
+#pragma unroll
+            for (int s = 0; s < SP; ++s) {
+                if constexpr (KEEP) {
+                    wa_raw[s] = choose(of_k, wk_raw[s][0], wq_raw[s][0]);
+                    wb_raw[s] = choose(of_k, wk_raw[s][1], wq_raw[s][1]);
+                } else {
+                    wa_raw[s] = wb_raw[s] = R{};
+                    const T *w = of_k ? wk : wq;
+                    if (weighted && on[s]) wa_raw[s] = load_raw<T, VEC>(w + at[s].a);
+                    if (weighted && on_b[s]) wb_raw[s] = load_raw<T, VEC>(w + at[s].b);
+                }
+            }
+            const float r = rsqrtf(lanes_sum(square, p.lanes) * inv_d + eps);
+            T *to = of_k ? ky + (long long)n * k_out_row : qy + (long long)n * q_out_row + (p.single ? 0 : i - 1) * D;
             if constexpr (!BWD) {
 #pragma unroll
                 for (int s = 0; s < SP; ++s) {
                     float wa[VEC], wb[VEC];
-                    expand<T, VEC>(of_k ? wk_raw[s][0] : wq_raw[s][0], wa);
-                    expand<T, VEC>(of_k ? wk_raw[s][1] : wq_raw[s][1], wb);
+                    expand<T, VEC>(wa_raw[s], wa);
+                    expand<T, VEC>(wb_raw[s], wb);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         a[s][e] *= r;
@@ -234,8 +273,8 @@ __global__ void __launch_bounds__(THREADS) qk_norm_kernel(const HeadArgs p)
 #pragma unroll
                 for (int s = 0; s < SP; ++s) {
                     float wa[VEC], wb[VEC];
-                    expand<T, VEC>(of_k ? wk_raw[s][0] : wq_raw[s][0], wa);
-                    expand<T, VEC>(of_k ? wk_raw[s][1] : wq_raw[s][1], wb);
+                    expand<T, VEC>(wa_raw[s], wa);
+                    expand<T, VEC>(wb_raw[s], wb);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         a[s][e] *= r;  // x r from here on
@@ -337,6 +376,7 @@ int check_args(const char *who, const cf_qk_norm *d)
                who, (long long)d->N, (long long)d->Hq, (long long)d->Hk, (long long)d->D);
     CF_REQUIRE(d->Hq % d->Hk == 0, CF_ERR_INVALID, "%s: %lld query heads do not share %lld key heads evenly", who, (long long)d->Hq, (long long)d->Hk);
     CF_REQUIRE(2 * d->P <= d->D, CF_ERR_INVALID, "%s: %lld pairs in heads of %lld", who, (long long)d->P, (long long)d->D);
+    CF_REQUIRE(d->q_row < (1ll << 31) && d->q_head < (1ll << 31) && d->k_row < (1ll << 31) && d->k_head < (1ll << 31), CF_ERR_RANGE, "%s: stride of 2^31", who);
     CF_REQUIRE(d->q_row >= 0 && d->q_head >= 0 && d->k_row >= 0 && d->k_head >= 0, CF_ERR_INVALID, "%s: negative stride", who);
     CF_REQUIRE((d->wq_head == 0 || d->wq_head == d->D) && (d->wk_head == 0 || d->wk_head == d->D), CF_ERR_INVALID, "%s: weights are (D) or (H, D)", who);
     CF_REQUIRE(d->N == 0 || (d->q && d->k), CF_ERR_INVALID, "%s: null pointer", who);
@@ -360,6 +400,7 @@ bool fits(const HeadArgs &a, int vec, bool backward)
     if (!aligned_to(d.q, bytes) || !aligned_to(d.k, bytes) || !aligned_to(a.q_out, bytes) || !aligned_to(a.k_out, bytes) || !aligned_to(d.wq, bytes) ||
         !aligned_to(d.wk, bytes))
         return false;
+    if (d.P > 0 && !aligned_to(d.waves, 16)) return false;
     return !backward || (aligned_to(a.gq_out, bytes) && aligned_to(a.gk_out, bytes));
 }
 
@@ -412,7 +453,7 @@ int launch_vec(HeadArgs a, void *gwq, void *gwk, cudaStream_t s)
     while (a.lanes < 32 && a.lanes < a.slots) a.lanes *= 2;
     const int sp = (a.slots + a.lanes - 1) / a.lanes;
     if (sp <= 1) return launch_sp<T, VEC, 1, BWD>(a, gwq, gwk, s);
-    if (sp <= 2) return launch_sp<T, VEC, 2, BWD>(a, gwq, gwk, s);  // (heads of up to 512: 64 slots of 8 values, 256 of 2)
+    if constexpr (VEC <= 4) if (sp <= 2) return launch_sp<T, VEC, 2, BWD>(a, gwq, gwk, s);  // (heads of up to 512: 64 slots of 8 values, 256 of 2)
     if constexpr (VEC == 1) return launch_sp<T, VEC, 8, BWD>(a, gwq, gwk, s);
     return fail(CF_ERR_RANGE, "cf_qk_norm: heads of %lld", (long long)a.d.D);
 }
@@ -420,6 +461,9 @@ int launch_vec(HeadArgs a, void *gwq, void *gwk, cudaStream_t s)
 template <class T, bool BWD>
 int launch(const HeadArgs &a, void *gwq, void *gwk, cudaStream_t s)
 {
+    if constexpr (sizeof(T) == 2 && !BWD) {
+        if (fits(a, 8, BWD)) return launch_vec<T, 8, BWD>(a, gwq, gwk, s);
+    }
     if (fits(a, 4, BWD)) return launch_vec<T, 4, BWD>(a, gwq, gwk, s);
     return launch_vec<T, 1, BWD>(a, gwq, gwk, s);
 }

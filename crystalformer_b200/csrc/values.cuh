@@ -92,19 +92,29 @@ template <> struct RawBytes<4> { using type = uint32_t; };
 template <> struct RawBytes<2> { using type = uint16_t; };
 template <class T, int VEC> using Raw = typename RawBytes<VEC * sizeof(T)>::type;
 template <class T, int VEC> __device__ __forceinline__ Raw<T, VEC> load_raw(const T *p) { return *reinterpret_cast<const Raw<T, VEC> *>(p); }
+__device__ __forceinline__ uint16_t choose(bool first, uint16_t a, uint16_t b) { return first ? a : b; }
+__device__ __forceinline__ uint32_t choose(bool first, uint32_t a, uint32_t b) { return first ? a : b; }
+__device__ __forceinline__ uint2 choose(bool first, const uint2 &a, const uint2 &b) { return make_uint2(first ? a.x : b.x, first ? a.y : b.y); }
+__device__ __forceinline__ uint4 choose(bool first, const uint4 &a, const uint4 &b)
+{
+    return make_uint4(first ? a.x : b.x, first ? a.y : b.y, first ? a.z : b.z, first ? a.w : b.w);  // (in registers: an address is not taken)
+}
+template <class T> __device__ __forceinline__ float value_of(uint32_t w) { return __uint_as_float(w); }  // of a word with one value
+template <> __device__ __forceinline__ float value_of<__nv_bfloat16>(uint32_t w) { return __uint_as_float(w << 16); }
+template <> __device__ __forceinline__ float value_of<__half>(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)w)); }
 template <class T, int VEC>
 __device__ __forceinline__ void expand(const Raw<T, VEC> &raw, float (&v)[VEC])
 {
-    if constexpr (VEC == 1 || sizeof(T) == 4) {
-        const T *t = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = to_float(t[i]);
+    if constexpr (VEC == 1) {
+        v[0] = value_of<T>(raw);
+    } else if constexpr (sizeof(T) == 4) {
+        v[0] = __uint_as_float(raw.x); v[1] = __uint_as_float(raw.y); v[2] = __uint_as_float(raw.z); v[3] = __uint_as_float(raw.w);
     } else {
-        const uint32_t *w = reinterpret_cast<const uint32_t *>(&raw);
-#pragma unroll
-        for (int i = 0; i < VEC / 2; ++i) {
-            const float2 f = unpack_two<T>(w[i]);
-            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        const float2 f = unpack_two<T>(raw.x), g = unpack_two<T>(raw.y);
+        v[0] = f.x; v[1] = f.y; v[2] = g.x; v[3] = g.y;
+        if constexpr (VEC == 8) {
+            const float2 h = unpack_two<T>(raw.z), i = unpack_two<T>(raw.w);
+            v[4] = h.x; v[5] = h.y; v[6] = i.x; v[7] = i.y;
         }
     }
 }
