@@ -7,7 +7,7 @@
 // 6 N D F operations forward, 12 backward and 4 to compute g and u again (keeping them costs 8 N F bytes each way in float32, which
 // take as long as the products up to D of about a thousand).  Forward: one kernel for both projections, the activation and the
 // product (tile_gemm.cuh, GLU_FORWARD), one for the projection back.  Backward: one kernel for g, u, dh and all that is element-wise
-// (GLU_BACKWARD), one for gx, one for both gate weights' gradients, one for gWd, and sums of columns for the biases.
+// (GLU_BACKWARD), one for the three products that give gx, gWg with gWu, and gWd, and one for the biases' sums.
 // 16-bit types: h, dg and du are rounded to the type once, as operands of the next product; all sums are float32.
 // Up to eight rows take no tiles (gated_rows.cuh): the weights are read once, and that is the time.
 #include <algorithm>
@@ -86,54 +86,37 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
     }
 }
 
-// ---- shares of a split contraction, added in their order --------------------------------------------------------------------------
-struct ShareArgs {
-    const float *partial;
-    int splits, N;
-    long long M;
-    void *out0, *out1;
-    long long rows0, row1, rows1, ld_out;
-    const void *bias;
-};
-template <class T>
-__global__ void __launch_bounds__(256) share_sum_kernel(const ShareArgs p)
-{
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const long long all = p.M * p.N;
-    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < all; at += (long long)gridDim.x * 256) {
-        const long long row = at / p.N;
-        const int col = (int)(at - row * p.N);
-        T *to;
-        if (row < p.rows0) to = static_cast<T *>(p.out0) + row * p.ld_out;
-        else if (row >= p.row1 && row < p.row1 + p.rows1) to = static_cast<T *>(p.out1) + (row - p.row1) * p.ld_out;
-        else continue;
-        float t = 0.f;
-#pragma unroll 4
-        for (int s = 0; s < p.splits; ++s) t += p.partial[s * all + at];
-        if (p.bias != nullptr) t += to_float(static_cast<const T *>(p.bias)[col]);
-        to[col] = from_float<T>(t);
-    }
-}
-
 // ---- sums of columns (the biases' gradients) --------------------------------------------------------------------------------------
-// Shares of the rows of a matrix: a block's eight warps take rows in turn, a lane VEC columns, and add up at the end.
-template <class T, int VEC>
-__global__ void __launch_bounds__(256) column_share_kernel(const T *x, long long rows, int cols, float *partial)
+// Of a matrix of rows in a type (gy) or of float32 sums of 32 rows each (dg and du): a block takes 32 VEC columns of a share of the
+// rows, its eight warps rows in turn; the block that brings a column group's last share adds the shares in their order.
+struct ColumnJob {
+    const void *x;
+    long long rows;
+    int cols, groups, shares;
+    float *partial;       // (shares, cols)
+    unsigned *tickets;    // per group
+    void *out0, *out1;    // columns [0, cols0), [col1, col1 + cols1)
+    int cols0, col1, cols1;
+};
+struct ColumnJobs {
+    ColumnJob j[2];
+};
+template <class T, class X, int VEC>
+__device__ __forceinline__ void sum_columns(const ColumnJob &job, int block)
 {
     __shared__ float part[8][32 * VEC];
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = (blockIdx.x * 32 + lane) * VEC;
-    const long long lo = rows * blockIdx.y / gridDim.y, hi = rows * (blockIdx.y + 1) / gridDim.y;
+    __shared__ bool last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = block % job.groups, share = block / job.groups, col = (group * 32 + lane) * VEC;
+    const long long lo = job.rows * share / job.shares, hi = job.rows * (share + 1) / job.shares;
+    const X *x = static_cast<const X *>(job.x);
     float sum[VEC], low[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[e] = low[e] = 0.f;
-    if (col < cols) {
+    if (col < job.cols) {
 #pragma unroll 4
         for (long long n = lo + warp; n < hi; n += 8) {
             float v[VEC];
-            load_values<T, VEC>(x + n * cols + col, v);
+            load_values<X, VEC>(x + n * job.cols + col, v);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) add_compensated(v[e], sum[e], low[e]);
         }
@@ -142,36 +125,36 @@ __global__ void __launch_bounds__(256) column_share_kernel(const T *x, long long
     for (int e = 0; e < VEC; ++e) part[warp][e * 32 + lane] = sum[e] + low[e];
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
-        const int at = (blockIdx.x * 32 + (i & 31)) * VEC + (i >> 5);
+        const int at = (group * 32 + (i & 31)) * VEC + (i >> 5);
         float t = 0.f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) t += part[w][i];
-        if (at < cols) partial[(long long)blockIdx.y * cols + at] = t;
+        if (at < job.cols) __stcg(job.partial + (long long)share * job.cols + at, t);
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(job.tickets + group, 1u) + 1u == (unsigned)job.shares;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+        const int at = group * 32 * VEC + i;
+        if (at >= job.cols) continue;
+        float t = 0.f;
+#pragma unroll 8
+        for (int s = 0; s < job.shares; ++s) t += __ldcg(job.partial + (long long)s * job.cols + at);
+        if (at < job.cols0) { if (job.out0 != nullptr) static_cast<T *>(job.out0)[at] = from_float<T>(t); }
+        else if (at >= job.col1 && at < job.col1 + job.cols1) { if (job.out1 != nullptr) static_cast<T *>(job.out1)[at - job.col1] = from_float<T>(t); }
     }
 }
-// Shares added: to fewer of them (`fewer`, gridDim.y of them), or to the columns' places in the gradients.
-template <class T>
-__global__ void __launch_bounds__(256) column_sum_kernel(const float *partial, long long shares, int cols, float *fewer, T *out0, int cols0, T *out1, int col1,
-                                                         int cols1)
+template <class T, int VEC>
+__global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__ ColumnJobs jobs)
 {
-    __shared__ float part[8][32];
     grid_launch_dependents();
     grid_dependency_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
-    const long long lo = shares * blockIdx.y / gridDim.y, hi = shares * (blockIdx.y + 1) / gridDim.y;
-    float t = 0.f;
-    if (col < cols) {
-#pragma unroll 8
-        for (long long s = lo + warp; s < hi; s += 8) t += partial[s * cols + col];
-    }
-    part[warp][lane] = t;
-    __syncthreads();
-    if (warp > 0 || col >= cols) return;
-#pragma unroll
-    for (int w = 1; w < 8; ++w) t += part[w][lane];
-    if (fewer != nullptr) fewer[(long long)blockIdx.y * cols + col] = t;
-    else if (col < cols0) { if (out0 != nullptr) out0[col] = from_float<T>(t); }
-    else if (col >= col1 && col < col1 + cols1) { if (out1 != nullptr) out1[col - col1] = from_float<T>(t); }
+    const int first = jobs.j[0].groups * jobs.j[0].shares;
+    if ((int)blockIdx.x < first) sum_columns<T, float, 4>(jobs.j[0], blockIdx.x);
+    else sum_columns<T, T, VEC>(jobs.j[1], blockIdx.x - first);
 }
 
 // ---- tensor maps ----------------------------------------------------------------------------------------------------------------------
@@ -216,7 +199,7 @@ struct Operand {
 
 // ---- launches ----------------------------------------------------------------------------------------------------------------------------
 template <class T, int MODE, int TN, bool PAIR>
-int launch_tiles(const Params &p, bool chained, cudaStream_t s)
+int launch_tiles(const ParamsOf<MODE> &p, bool chained, cudaStream_t s)
 {
     using S = Shape<T, MODE, TN, PAIR>;
     static thread_local int resident[64] = {};  // blocks that the GPU holds at a time (0: not asked yet)
@@ -247,7 +230,8 @@ int launch_tiles(const Params &p, bool chained, cudaStream_t s)
         }
         blocks = PAIR ? std::min(2 * clusters, sm_count()) : sm_count();
     }
-    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
+    long long tiles = 0;
+    for (int i = 0; i < p.count; ++i) tiles += p.q[i].tiles;
     cfg.gridDim = dim3((unsigned)std::min<long long>(PAIR ? 2 * tiles : tiles, blocks));
     cfg.numAttrs = chained && chained_launches_enabled() ? 2 : 1;
     if (cudaLaunchKernelEx(&cfg, tile_kernel<T, MODE, TN, PAIR>, p) != cudaSuccess) return launch_status("tile_kernel");
@@ -257,7 +241,9 @@ int launch_tiles(const Params &p, bool chained, cudaStream_t s)
 // Blocks of a grid-stride kernel over `work` units of one thread each.
 unsigned stride_blocks(long long work) { return (unsigned)std::max(1ll, std::min((work + 255) / 256, (long long)sm_count() * 8)); }
 
-// C (M, N) = sum over parts of A B^T; where splitting pays, float32 shares through `partial`.
+int blocks_of(long long K) { return (int)((K + TK - 1) / TK); }
+
+// C (M, N) = sum over parts of A B^T.
 struct Linear {
     Operand a[2], b[2];
     bool a_across[2], b_across[2];
@@ -268,82 +254,127 @@ struct Linear {
     void *out0, *out1;
     long long rows0, row1, rows1, ld_out;
     const void *bias;
+    int splits;
 };
 
-int blocks_of(long long K) { return (int)((K + TK - 1) / TK); }
-
-// Width of the tiles, one block or a pair of them to a tile, and number of shares: the cheapest of the kernel's rounds (blocks of the
-// contraction, and what a tile costs beside them) and of the shares' way through memory.  Unit: 256 clocks, the products of
-// 128 x 128 x 64 values of 16 bits.
+// How the products of one launch are cut: width of the tiles, one block or a pair of them to a tile, and into how many shares each
+// contraction.  Shares are as long as `length` blocks at most, so that the tiles of all products take about as long; the cheapest
+// length by the rounds of the launch (blocks of the contraction, and what a tile costs beside them) and by the shares' way through
+// memory.  Unit: 256 clocks, the products of 128 x 128 x 64 values of 16 bits.
+struct Size {
+    long long M;
+    int N, blocks;
+};
 struct Cut {
     int tn;
     bool pair;
-    int splits;
+    int splits[LINEAR_COUNT];
+    size_t floats, tickets;  // of all shares, of all warps' parts of split tiles
 };
 template <class T>
-Cut linear_cut(long long M, int N, int blocks)
+Cut find_cut(const Size *sizes, int count)
 {
-    // a block of the contraction of a 16-bit type: its products, or (tiles of one block) what L2 delivers; of float32: six products
+    // a block of the contraction of a 16-bit type: its products, or what L2 delivers; of float32: six products
     struct Kind { int tn; bool pair; double one, six; };
-    constexpr Kind kinds[] = {{256, true, 2.0, 12.5}, {128, true, 1.15, 6.6}, {128, false, 1.7, 7.2}, {64, false, 1.2, 4.4}};
+    constexpr Kind kinds[] = {{256, true, 3.4, 12.5}, {128, true, 3.2, 8.0}, {128, false, 3.2, 9.0}, {64, false, 2.2, 5.0}};
     constexpr bool wide = pieces_of<T> > 1;
     const double sms = sm_count();
-    Cut best{128, false, 1};
+    int most = 1;
+    for (int i = 0; i < count; ++i) most = std::max(most, sizes[i].blocks);
+    Cut best{};
     double least = 1e300;
     for (const Kind &k : kinds) {
-        const double tiles = (double)((M + (k.pair ? 255 : 127)) / (k.pair ? 256 : 128)) * ((N + k.tn - 1) / k.tn);
-        for (int sp = 1; sp <= 64 && sp <= blocks; sp = sp < 4 ? sp + 1 : sp + sp / 4) {
-            const double rounds = std::ceil(tiles * sp / (k.pair ? std::floor(sms / 2) : sms));
-            // a tile's start and the last one's epilogue: some 8 units; shares: a launch, and 8 bytes a value at 13 KB a unit
-            const double cost = rounds * std::ceil((double)blocks / sp) * (wide ? k.six : k.one) + 8.0 + 3.0 * rounds +
-                                (sp > 1 ? 16.0 + (double)sp * M * N * 8.0 / 1e6 : 0.0);
+        const int tm = k.pair ? 2 * TM : TM;
+        const double at_once = k.pair ? std::floor(sms / 2) : sms, block = wide ? k.six : k.one;
+        for (int length = most; length >= 1; length = length > 4 ? length * 3 / 4 : length - 1) {
+            Cut c{k.tn, k.pair, {}, 0, 0};
+            double tiles = 0, work = 0, longest = 0;
+            for (int i = 0; i < count; ++i) {
+                const Size &z = sizes[i];
+                const int splits = (z.blocks + length - 1) / length;
+                const double n = (double)((z.M + tm - 1) / tm) * ((z.N + k.tn - 1) / k.tn);
+                const double each = std::ceil((double)z.blocks / splits) * block + 4.0 + (splits > 1 ? 1.0 : 0.0);
+                c.splits[i] = splits;
+                tiles += n * splits;
+                work += n * splits * each;
+                longest = std::max(longest, each);
+                if (splits > 1) {
+                    c.floats += (size_t)n * splits * tm * k.tn;
+                    c.tickets += (size_t)n * (k.pair ? 2 : 1) * EPILOGUE_WARPS;
+                }
+            }
+            // rounds of tiles of about the same length; 8 bytes a value of a share, at 900 KB a unit
+            const double cost = std::max(std::ceil(tiles / at_once) * (work / tiles), longest) + 10.0 + (double)c.floats * 8.0 / 9e5;
             if (cost < least * 0.99) {
                 least = cost;
-                best = {k.tn, k.pair, sp};
+                best = c;
             }
         }
     }
     return best;
 }
 
+// The cut of the last sizes asked for is kept, per thread: it costs some microseconds, and a call asks twice (for its workspace's size).
 template <class T>
-size_t linear_partial(long long M, int N, int blocks)
+Cut linear_cut(const Size *sizes, int count)
 {
-    const Cut c = linear_cut<T>(M, N, blocks);
-    return c.splits > 1 ? (size_t)c.splits * M * N : 0;
+    struct Last {
+        Size sizes[LINEAR_COUNT];
+        int sms = 0;
+        Cut cut;
+    };
+    static thread_local Last last[LINEAR_COUNT];
+    Last &l = last[count - 1];
+    bool same = l.sms == sm_count();
+    for (int i = 0; i < count; ++i) same = same && l.sizes[i].M == sizes[i].M && l.sizes[i].N == sizes[i].N && l.sizes[i].blocks == sizes[i].blocks;
+    if (!same) {
+        l.cut = find_cut<T>(sizes, count);
+        l.sms = sm_count();
+        std::copy(sizes, sizes + count, l.sizes);
+    }
+    return l.cut;
 }
 
 template <class T>
-int run_linear(const Linear &l, float *partial, cudaStream_t s)
+int run_linear(const Linear *products, int count, const Cut &cut, float *partial, unsigned *tickets, cudaStream_t s)
 {
-    Params p{};
-    p.blocks0 = blocks_of(l.K[0]);
-    p.blocks = p.blocks0 + (l.parts > 1 ? blocks_of(l.K[1]) : 0);
-    const Cut cut = linear_cut<T>(l.M, l.N, p.blocks);
-    for (int i = 0; i < l.parts; ++i) {
-        p.a_across[i] = l.a_across[i];
-        p.b_across[i] = l.b_across[i];
-        int rc = encode<T>(&p.a[i], l.a[i].x, l.a[i].rows, l.a[i].cols, l.a_across[i] ? TK : TM);
-        if (rc == CF_OK) rc = encode<T>(&p.b[i], l.b[i].x, l.b[i].rows, l.b[i].cols, l.b_across[i] ? TK : cut.pair ? cut.tn / 2 : cut.tn);
-        if (rc != CF_OK) return rc;
-    }
-    p.M = l.M;
-    p.N = l.N;
+    if (count == 0) return CF_OK;
     const int tm = cut.pair ? 2 * TM : TM;
-    p.m_tiles = (int)((l.M + tm - 1) / tm);
-    p.n_tiles = (l.N + cut.tn - 1) / cut.tn;
-    p.splits = cut.splits;
-    p.out0 = l.out0; p.out1 = l.out1;
-    p.rows0 = l.rows0; p.row1 = l.row1; p.rows1 = l.rows1; p.ld_out = l.ld_out;
-    p.bias = l.bias;
-    p.partial = cut.splits > 1 ? partial : nullptr;
+    ParamsOf<LINEAR> p{};
+    p.count = count;
     p.status = wait_status();
-    const int rc = cut.tn == 256 ? launch_tiles<T, LINEAR, 256, true>(p, true, s) : cut.pair ? launch_tiles<T, LINEAR, 128, true>(p, true, s) :
-                   cut.tn == 128 ? launch_tiles<T, LINEAR, 128, false>(p, true, s) : launch_tiles<T, LINEAR, 64, false>(p, true, s);
-    if (rc != CF_OK || cut.splits == 1) return rc;
-    const ShareArgs sum{partial, cut.splits, l.N, l.M, l.out0, l.out1, l.rows0, l.row1, l.rows1, l.ld_out, l.bias};
-    if (launch_chained(share_sum_kernel<T>, dim3(stride_blocks(l.M * l.N)), dim3(256), 0, s, true, sum) != cudaSuccess) return launch_status("share_sum_kernel");
-    return launch_status("share_sum_kernel");
+    for (int i = 0; i < count; ++i) {
+        const Linear &l = products[i];
+        Problem &q = p.q[i];
+        for (int part = 0; part < l.parts; ++part) {
+            q.a_across[part] = l.a_across[part];
+            q.b_across[part] = l.b_across[part];
+            int rc = encode<T>(&q.a[part], l.a[part].x, l.a[part].rows, l.a[part].cols, l.a_across[part] ? TK : TM);
+            if (rc == CF_OK)
+                rc = encode<T>(&q.b[part], l.b[part].x, l.b[part].rows, l.b[part].cols, l.b_across[part] ? TK : cut.pair ? cut.tn / 2 : cut.tn);
+            if (rc != CF_OK) return rc;
+        }
+        q.blocks0 = blocks_of(l.K[0]);
+        q.blocks = q.blocks0 + (l.parts > 1 ? blocks_of(l.K[1]) : 0);
+        q.M = l.M;
+        q.N = l.N;
+        q.m_tiles = (int)((l.M + tm - 1) / tm);
+        q.n_tiles = (l.N + cut.tn - 1) / cut.tn;
+        q.splits = l.splits;
+        q.tiles = (long long)q.m_tiles * q.n_tiles * q.splits;
+        CF_REQUIRE(q.tiles < (1ll << 31), CF_ERR_RANGE, "cf_gated_ffn: %lld tiles", q.tiles);
+        q.out0 = l.out0; q.out1 = l.out1;
+        q.rows0 = l.rows0; q.row1 = l.row1; q.rows1 = l.rows1; q.ld_out = l.ld_out;
+        q.bias = l.bias;
+        if (q.splits > 1) {
+            q.partial = partial;
+            q.tickets = tickets;
+            partial += (size_t)q.tiles * tm * cut.tn;
+            tickets += (size_t)q.m_tiles * q.n_tiles * (cut.pair ? 2 : 1) * EPILOGUE_WARPS;
+        }
+    }
+    return cut.tn == 256 ? launch_tiles<T, LINEAR, 256, true>(p, true, s) : cut.pair ? launch_tiles<T, LINEAR, 128, true>(p, true, s) :
+           cut.tn == 128 ? launch_tiles<T, LINEAR, 128, false>(p, true, s) : launch_tiles<T, LINEAR, 64, false>(p, true, s);
 }
 
 // ---- plans: where the operands of a call lie ------------------------------------------------------------------------------------------------
@@ -357,6 +388,10 @@ struct Plan {
     long long Fp;
     Operand x, wg, wu, wd, gy, h, dg, du;
     float *partial, *sums = nullptr;  // sums: of the columns of dg and du, 32 rows each
+    float *column_shares = nullptr;
+    unsigned *tickets;                // of split products, then of column groups
+    size_t ticket_words = 0;
+    Cut cut;
     size_t bytes;
     PackJobs jobs{};
     int job_count = 0;
@@ -382,19 +417,23 @@ struct Plan {
         if (backward) gy = place(c, gy_src, d.N, d.D, d.D);
         P *hm = c.take<P>((size_t)NP * d.N * Fp);
         h = {{hm, Fp, d.N * Fp}, d.N, d.F};
-        size_t floats = 0;
         if (!backward) {
-            floats = linear_partial<T>(d.N, (int)d.D, blocks_of(d.F));
+            const Size y{d.N, (int)d.D, blocks_of(d.F)};
+            cut = linear_cut<T>(&y, 1);
         } else {
             P *g = c.take<P>((size_t)NP * d.N * 2 * Fp);
             dg = {{g, 2 * Fp, d.N * 2 * Fp}, d.N, d.F};
             du = {{g ? g + Fp : g, 2 * Fp, d.N * 2 * Fp}, d.N, d.F};
-            const int rows = blocks_of(d.N);
-            floats = std::max<size_t>({linear_partial<T>(d.N, (int)d.D, 2 * blocks_of(d.F)), linear_partial<T>(2 * Fp, (int)d.D, rows),
-                               linear_partial<T>(d.D, (int)d.F, rows), (size_t)(COLUMN_SHARES * std::max<long long>(2 * Fp, d.D))});
+            const int rows = blocks_of(d.N);  // (a call that leaves a gradient out cuts the others the same way)
+            const Size every[3] = {{d.N, (int)d.D, 2 * blocks_of(d.F)}, {2 * Fp, (int)d.D, rows}, {d.D, (int)d.F, rows}};
+            cut = linear_cut<T>(every, 3);
             sums = c.take<float>((size_t)((d.N + 31) / 32) * 2 * Fp);
+            column_shares = c.take<float>((size_t)COLUMN_SHARES * (2 * Fp + d.D));
+            ticket_words = (size_t)(2 * Fp + d.D);
         }
-        partial = c.take<float>(floats);
+        partial = c.take<float>(cut.floats);
+        ticket_words += cut.tickets;
+        tickets = c.take<unsigned>(ticket_words);
         bytes = c.used;
     }
 };
@@ -414,7 +453,11 @@ int run_glu(const Plan<T> &plan, bool backward, bool sums, cudaStream_t s)
 {
     const cf_gated_ffn &d = plan.d;
     constexpr bool wide = pieces_of<T> > 1;
-    Params p{};
+    ParamsOf<GLU_FORWARD> p{};
+    Problem &q = p.q[0];
+    p.count = 1;
+    p.clear = plan.tickets;
+    p.clear_words = (int)plan.ticket_words;
     // Tiles of pairs (256 x 128; backward in three pieces, whose sums must fit registers, 256 x 64) or of single blocks (128 x 64): the
     // cheaper by rounds times products, single blocks' bound by L2 (16 bits).
     const int pair_tn = wide && backward ? 64 : 128;
@@ -424,25 +467,27 @@ int run_glu(const Plan<T> &plan, bool backward, bool sums, cudaStream_t s)
     const bool pair = rounds(256, pair_tn, std::floor(sms / 2)) * pair_tn * (blocks + 2) < rounds(128, 64, sms) * 64 * (blocks + 2) * (wide ? 1.1 : 1.4);
     const int tn = pair ? pair_tn : 64, tm = pair ? 2 * TM : TM;
     const int of_x = backward ? 1 : 0;
-    p.blocks0 = blocks_of(d.D);
-    p.blocks = backward ? 2 * p.blocks0 : p.blocks0;
-    int rc = encode<T>(&p.a[of_x], plan.x.x, d.N, d.D, TM);
-    if (rc == CF_OK) rc = encode<T>(&p.b[1], plan.wg.x, d.F, d.D, tn);
-    if (rc == CF_OK) rc = encode<T>(&p.b[2], plan.wu.x, d.F, d.D, tn);
+    q.blocks0 = blocks_of(d.D);
+    q.blocks = backward ? 2 * q.blocks0 : q.blocks0;
+    int rc = encode<T>(&q.a[of_x], plan.x.x, d.N, d.D, TM);
+    if (rc == CF_OK) rc = encode<T>(&q.b[1], plan.wg.x, d.F, d.D, tn);
+    if (rc == CF_OK) rc = encode<T>(&q.b[2], plan.wu.x, d.F, d.D, tn);
     if (backward) {
-        if (rc == CF_OK) rc = encode<T>(&p.a[0], plan.gy.x, d.N, d.D, TM);
-        if (rc == CF_OK) rc = wide ? encode<T>(&p.b[0], plan.wd.x, d.F, d.D, pair ? tn / 2 : tn) : encode<T>(&p.b[0], plan.wd.x, d.D, d.F, TK);
-        p.b_across[0] = !wide;
+        if (rc == CF_OK) rc = encode<T>(&q.a[0], plan.gy.x, d.N, d.D, TM);
+        if (rc == CF_OK) rc = wide ? encode<T>(&q.b[0], plan.wd.x, d.F, d.D, pair ? tn / 2 : tn) : encode<T>(&q.b[0], plan.wd.x, d.D, d.F, TK);
+        q.b_across[0] = !wide;
         p.dg = plan.dg.x;
         p.du = plan.du.x;
         p.sums = sums ? plan.sums : nullptr;
     }
     if (rc != CF_OK) return rc;
-    p.m_tiles = (int)((d.N + tm - 1) / tm);
-    p.n_tiles = (int)((d.F + tn - 1) / tn);
-    p.splits = 1;
-    p.M = d.N;
-    p.N = (int)d.F;
+    q.m_tiles = (int)((d.N + tm - 1) / tm);
+    q.n_tiles = (int)((d.F + tn - 1) / tn);
+    q.splits = 1;
+    q.tiles = (long long)q.m_tiles * q.n_tiles;
+    CF_REQUIRE(q.tiles < (1ll << 31), CF_ERR_RANGE, "cf_gated_ffn: %lld tiles", q.tiles);
+    q.M = d.N;
+    q.N = (int)d.F;
     p.bias_gate = d.b_gate;
     p.bias_up = d.b_up;
     p.act = d.activation;
@@ -469,34 +514,42 @@ int forward(const cf_gated_ffn &d, void *y, void *workspace, cudaStream_t s)
     l.M = d.N; l.N = (int)d.D;
     l.out0 = y; l.rows0 = d.N; l.row1 = d.N; l.ld_out = d.D;
     l.bias = d.b_down;
-    return run_linear<T>(l, plan.partial, s);
-}
-
-// The shares of columns in `from` (through `fewer` where they are many) to their places.
-template <class T>
-int column_sums(const float *from, long long shares, int cols, float *fewer, T *out0, int cols0, T *out1, int col1, int cols1, cudaStream_t s)
-{
-    const unsigned groups = (unsigned)(cols + 31) / 32;
-    if (shares > 256) {
-        const unsigned to = (unsigned)std::min<long long>(COLUMN_SHARES, shares / 64);
-        launch_chained(column_sum_kernel<T>, dim3(groups, to), dim3(256), 0, s, true, from, shares, cols, fewer, out0, cols0, out1, col1, cols1);
-        from = fewer;
-        shares = to;
-    }
-    launch_chained(column_sum_kernel<T>, dim3(groups), dim3(256), 0, s, true, from, shares, cols, static_cast<float *>(nullptr), out0, cols0, out1, col1, cols1);
-    return launch_status("column_sum_kernel");
+    l.splits = plan.cut.splits[0];
+    return run_linear<T>(&l, 1, plan.cut, plan.partial, plan.tickets, s);
 }
 
 template <class T>
-int row_sums(const T *x, long long rows, int cols, float *partial, T *out, cudaStream_t s)
+int run_columns(const Plan<T> &plan, const cf_gated_ffn_grads &g, cudaStream_t s)
 {
+    const cf_gated_ffn &d = plan.d;
+    const int D = (int)d.D, F = (int)d.F, Fp = (int)plan.Fp;
     constexpr int VEC = 16 / sizeof(T);
-    const bool wide = cols % VEC == 0 && aligned_to(x, 16);
-    const unsigned groups = (unsigned)(cols + (wide ? 32 * VEC : 32) - 1) / (wide ? 32 * VEC : 32);
-    const unsigned shares = (unsigned)std::max(1ll, std::min<long long>(COLUMN_SHARES, rows / 32));
-    if (wide) launch_chained(column_share_kernel<T, VEC>, dim3(groups, shares), dim3(256), 0, s, true, x, rows, cols, partial);
-    else launch_chained(column_share_kernel<T, 1>, dim3(groups, shares), dim3(256), 0, s, true, x, rows, cols, partial);
-    return column_sums<T>(partial, shares, cols, nullptr, out, cols, nullptr, cols, 0, s);
+    const bool wide = D % VEC == 0 && aligned_to(g.gy, 16);
+    ColumnJobs jobs{};
+    auto place = [&](ColumnJob &j, const void *x, long long rows, int cols, int vec, float *partial, unsigned *tickets) {
+        j.x = x; j.rows = rows; j.cols = cols;
+        j.groups = (cols + 32 * vec - 1) / (32 * vec);
+        // (enough blocks to fill the GPU, of 32 rows at least, few enough for the last one to add up)
+        j.shares = (int)std::max(1ll, std::min<long long>({(long long)COLUMN_SHARES, rows / 32, std::max(1ll, 6ll * sm_count() / j.groups)}));
+        j.partial = partial; j.tickets = tickets;
+    };
+    unsigned *tickets = plan.tickets + plan.cut.tickets;
+    if (g.b_gate || g.b_up) {
+        ColumnJob &j = jobs.j[0];
+        place(j, plan.sums, (d.N + 31) / 32, 2 * Fp, 4, plan.column_shares, tickets);
+        j.out0 = g.b_gate; j.cols0 = F;
+        j.out1 = g.b_up; j.col1 = Fp; j.cols1 = F;
+    }
+    if (g.b_down) {
+        ColumnJob &j = jobs.j[1];
+        place(j, g.gy, d.N, D, wide ? VEC : 1, plan.column_shares + (size_t)COLUMN_SHARES * 2 * Fp, tickets + 2 * Fp);
+        j.out0 = g.b_down; j.cols0 = D; j.col1 = D;
+    }
+    const int blocks = jobs.j[0].groups * jobs.j[0].shares + jobs.j[1].groups * jobs.j[1].shares;
+    if (blocks == 0) return CF_OK;
+    if (wide) launch_chained(column_sum_kernel<T, VEC>, dim3(blocks), dim3(256), 0, s, true, jobs);
+    else launch_chained(column_sum_kernel<T, 1>, dim3(blocks), dim3(256), 0, s, true, jobs);
+    return launch_status("column_sum_kernel");
 }
 
 template <class T>
@@ -508,8 +561,10 @@ int backward(const cf_gated_ffn &d, const cf_gated_ffn_grads &g, void *workspace
     if (rc != CF_OK) return rc;
     const int D = (int)d.D, F = (int)d.F;
     const long long Fp = plan.Fp;
+    Linear products[LINEAR_COUNT] = {};
+    int count = 0;
     if (g.x) {
-        Linear l{};
+        Linear &l = products[count++];
         l.a[0] = plan.dg; l.b[0] = plan.wg;
         l.a[1] = plan.du; l.b[1] = plan.wu;
         l.b_across[0] = l.b_across[1] = true;
@@ -517,10 +572,10 @@ int backward(const cf_gated_ffn &d, const cf_gated_ffn_grads &g, void *workspace
         l.K[0] = l.K[1] = F;
         l.M = d.N; l.N = D;
         l.out0 = g.x; l.rows0 = d.N; l.row1 = d.N; l.ld_out = D;
-        if ((rc = run_linear<T>(l, plan.partial, s)) != CF_OK) return rc;
+        l.splits = plan.cut.splits[0];
     }
     if (g.w_gate || g.w_up) {  // one product for both: rows [0, F) and [Fp, Fp + F)
-        Linear l{};
+        Linear &l = products[count++];
         l.a[0] = {plan.dg.x, d.N, 2 * Fp}; l.b[0] = plan.x;
         l.a_across[0] = l.b_across[0] = true;
         l.parts = 1;
@@ -529,24 +584,20 @@ int backward(const cf_gated_ffn &d, const cf_gated_ffn_grads &g, void *workspace
         l.out0 = g.w_gate; l.rows0 = g.w_gate ? F : 0;
         l.out1 = g.w_up; l.row1 = Fp; l.rows1 = g.w_up ? F : 0;
         l.ld_out = D;
-        if ((rc = run_linear<T>(l, plan.partial, s)) != CF_OK) return rc;
+        l.splits = plan.cut.splits[1];
     }
     if (g.w_down) {
-        Linear l{};
+        Linear &l = products[count++];
         l.a[0] = plan.gy; l.b[0] = plan.h;
         l.a_across[0] = l.b_across[0] = true;
         l.parts = 1;
         l.K[0] = d.N;
         l.M = D; l.N = F;
         l.out0 = g.w_down; l.rows0 = D; l.row1 = D; l.ld_out = F;
-        if ((rc = run_linear<T>(l, plan.partial, s)) != CF_OK) return rc;
+        l.splits = plan.cut.splits[2];
     }
-    if (g.b_gate || g.b_up) {
-        rc = column_sums<T>(plan.sums, (d.N + 31) / 32, (int)(2 * Fp), plan.partial, static_cast<T *>(g.b_gate), F, static_cast<T *>(g.b_up), (int)Fp, F, s);
-        if (rc != CF_OK) return rc;
-    }
-    if (g.b_down) rc = row_sums<T>(static_cast<const T *>(g.gy), d.N, D, plan.partial, static_cast<T *>(g.b_down), s);
-    return rc;
+    if ((rc = run_linear<T>(products, count, plan.cut, plan.partial, plan.tickets, s)) != CF_OK) return rc;
+    return run_columns(plan, g, s);
 }
 
 int check_args(const char *who, const cf_gated_ffn *d)

@@ -1,7 +1,8 @@
 // The tile products of the gated feed-forward on the fifth-generation tensor cores, in three modes:
 //
-//   LINEAR        C = A0 B0^T [+ A1 B1^T]                       epilogue: bias, stored in the type of the call; or float32 shares of a
-//                                                               split contraction, which a second kernel adds
+//   LINEAR        C = A0 B0^T [+ A1 B1^T]                       epilogue: bias, stored in the type of the call; of a split contraction
+//                                                               float32 shares, added by whoever brings a tile's last.  Up to three
+//                                                               products in one launch
 //   GLU_FORWARD   g = X Wg^T, u = X Wu^T                        epilogue: h = act(g + bg) (u + bu)
 //   GLU_BACKWARD  dh = Gy Wd, then the same                     epilogue: h, dg = dh u act'(g), du = dh act(g), sums of columns of 32 rows
 //
@@ -48,27 +49,40 @@ struct Planes {
     long long ld, plane;
 };
 
-struct Params {
-    // LINEAR: a[0] with b[0], a[1] with b[1]; GLU: x with b[1] (gate) and b[2] (up), backward: gy = a[0] with b[0] (down), x = a[1]
+// One product.  LINEAR: a[0] with b[0], a[1] with b[1]; GLU: x with b[1] (gate) and b[2] (up), backward: gy = a[0] with b[0] (down),
+// x = a[1].
+struct Problem {
     CUtensorMap a[2], b[3];
     int a_across[2], b_across[2];  // per part: the contraction runs across the rows of the operand
     int blocks0, blocks;      // of the contraction: of the first part, of both
     int m_tiles, n_tiles, splits;  // m_tiles: of 128 rows, or 256 of a pair
-    long long M;
     int N;
-    // GLU
-    const void *bias_gate, *bias_up;
-    int act;
-    Planes h, dg, du;
-    int padded;               // columns that h, dg and du have memory for, a multiple of 16
-    float *sums;              // or null: (32 rows each, 2 padded) sums of the columns of dg and du
+    long long M, tiles;       // tiles = m_tiles n_tiles splits
     // LINEAR: rows [0, rows0) to out0, rows [row1, row1 + rows1) to out1
     void *out0, *out1;
     long long rows0, row1, rows1, ld_out;
     const void *bias;
-    float *partial;           // (splits, M, N) instead
-    unsigned *status;
+    // splits > 1: every share of a tile, and how many of a warp's part of it are there (zero before); who brings the last adds them
+    float *partial;
+    unsigned *tickets;
 };
+
+template <int COUNT>
+struct Params {
+    Problem q[COUNT];
+    int count;
+    unsigned *clear;          // words that GLU sets to zero, for the kernels behind it
+    int clear_words;
+    unsigned *status;
+    // GLU
+    const void *bias_gate, *bias_up;
+    int act;
+    int padded;               // columns that h, dg and du have memory for, a multiple of 16
+    Planes h, dg, du;
+    float *sums;              // or null: (32 rows each, 2 padded) sums of the columns of dg and du
+};
+constexpr int LINEAR_COUNT = 3;  // products that one launch may have
+template <int MODE> using ParamsOf = Params<MODE == LINEAR ? LINEAR_COUNT : 1>;
 
 template <class T, int MODE, int TN, bool PAIR>
 struct Shape {
@@ -203,7 +217,7 @@ __device__ __forceinline__ float column_sum(const float (&v)[16], int lane)
 
 // The epilogue of 16 columns of a warp's 32 rows: v[acc][.] are the accumulators' values of this lane's row.
 template <class T, int MODE, int ACT>
-__device__ __forceinline__ void finish_glu(const Params &p, long long row, int col, const float *bias, float (&v)[MODE == GLU_FORWARD ? 2 : 3][16])
+__device__ __forceinline__ void finish_glu(const Params<1> &p, long long row, int col, const float *bias, float (&v)[MODE == GLU_FORWARD ? 2 : 3][16])
 {
     if (bias != nullptr) {
         add_16(bias, v[0]);
@@ -225,13 +239,13 @@ __device__ __forceinline__ void finish_glu(const Params &p, long long row, int c
             const int lane = threadIdx.x & 31;
             const float du = column_sum(v[1], lane), dg = column_sum(v[2], lane);  // (rows behind the last have dh = 0)
             float *to = p.sums + (row >> 5) * (2ll * p.padded) + col + (lane >> 1);
-            if ((lane & 1) == 0 && (row & ~31ll) < p.M) {
+            if ((lane & 1) == 0 && (row & ~31ll) < p.q[0].M) {
                 to[0] = dg;
                 to[p.padded] = du;
             }
         }
     }
-    if (row >= p.M) return;
+    if (row >= p.q[0].M) return;
     store_planes<T>(p.h, row, col, v[0]);
     if constexpr (MODE == GLU_BACKWARD) {
         store_planes<T>(p.du, row, col, v[1]);
@@ -239,26 +253,26 @@ __device__ __forceinline__ void finish_glu(const Params &p, long long row, int c
     }
 }
 
-template <class T, int MODE, int COUNT>
-__device__ __forceinline__ void finish(const Params &p, int split, long long row, int col, const float *bias, float (&v)[COUNT][16])
+template <class T>
+__device__ __forceinline__ void finish_linear(const Problem &q, long long row, int col, const float *bias, float (&v)[16])
 {
-    if (col >= p.N) return;
+    if (row >= q.M || col >= q.N) return;
+    if (bias != nullptr) add_16(bias, v);
+    T *to;
+    if (row < q.rows0) to = static_cast<T *>(q.out0) + row * q.ld_out;
+    else if (row >= q.row1 && row < q.row1 + q.rows1) to = static_cast<T *>(q.out1) + (row - q.row1) * q.ld_out;
+    else return;
+    to += col;
+    store_run<T>(to, q.N - col, (reinterpret_cast<uintptr_t>(to) & 31) == 0, v);
+}
+
+template <class T, int MODE, int COUNT>
+__device__ __forceinline__ void finish(const ParamsOf<MODE> &p, const Problem &q, long long row, int col, const float *bias, float (&v)[COUNT][16])
+{
     if constexpr (MODE == LINEAR) {
-        if (row >= p.M) return;
-        const int room = p.N - col;
-        if (p.partial != nullptr) {
-            float *to = p.partial + ((long long)split * p.M + row) * p.N + col;
-            store_run<float>(to, room, (reinterpret_cast<uintptr_t>(to) & 31) == 0, v[0]);
-            return;
-        }
-        if (bias != nullptr) add_16(bias, v[0]);
-        T *to;
-        if (row < p.rows0) to = static_cast<T *>(p.out0) + row * p.ld_out;
-        else if (row >= p.row1 && row < p.row1 + p.rows1) to = static_cast<T *>(p.out1) + (row - p.row1) * p.ld_out;
-        else return;
-        to += col;
-        store_run<T>(to, room, (reinterpret_cast<uintptr_t>(to) & 31) == 0, v[0]);
+        finish_linear<T>(q, row, col, bias, v[0]);
     } else {
+        if (col >= q.N) return;
         if (p.act == SILU) finish_glu<T, MODE, SILU>(p, row, col, bias, v);
         else if (p.act == GELU) finish_glu<T, MODE, GELU>(p, row, col, bias, v);
         else finish_glu<T, MODE, RELU>(p, row, col, bias, v);
@@ -266,24 +280,31 @@ __device__ __forceinline__ void finish(const Params &p, int split, long long row
 }
 
 struct Tile {
+    int q;  // which product
     int m, n, split;
     int k_lo, k_hi;
 };
-__device__ __forceinline__ Tile tile_of(const Params &p, long long t)
+template <int COUNT>
+__device__ __forceinline__ Tile tile_of(const Params<COUNT> &p, long long t)
 {
     // (columns run fastest: neighbours share rows of A, which are many, and the whole of B, which is small, stays in L2)
     Tile x;
-    x.n = (int)(t % p.n_tiles);
-    t /= p.n_tiles;
-    x.m = (int)(t % p.m_tiles);
-    x.split = (int)(t / p.m_tiles);
-    x.k_lo = (int)((long long)p.blocks * x.split / p.splits);
-    x.k_hi = (int)((long long)p.blocks * (x.split + 1) / p.splits);
+    x.q = 0;
+    if constexpr (COUNT > 1) {
+        while (x.q + 1 < p.count && t >= p.q[x.q].tiles) t -= p.q[x.q++].tiles;
+    }
+    const Problem &q = p.q[x.q];
+    const unsigned at = (unsigned)t, n_tiles = q.n_tiles, m_tiles = q.m_tiles;  // (a launch has fewer than 2^31 tiles)
+    x.n = (int)(at % n_tiles);
+    x.m = (int)(at / n_tiles % m_tiles);
+    x.split = (int)(at / n_tiles / m_tiles);
+    x.k_lo = (int)((long long)q.blocks * x.split / q.splits);
+    x.k_hi = (int)((long long)q.blocks * (x.split + 1) / q.splits);
     return x;
 }
 
 template <class T, int MODE, int TN, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ Params p)
+__global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ ParamsOf<MODE> p)
 {
     using namespace tc5;
     using S = Shape<T, MODE, TN, PAIR>;
@@ -317,10 +338,14 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + S::MISC + 232);
     grid_launch_dependents();
     grid_dependency_wait();
-    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits;
+    long long tiles = 0;
+    for (int i = 0; i < p.count; ++i) tiles += p.q[i].tiles;
+    if constexpr (MODE != LINEAR) {
+        for (int i = blockIdx.x * THREADS + threadIdx.x; i < p.clear_words; i += gridDim.x * THREADS) p.clear[i] = 0u;
+    }
     const long long first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
     // whether a block of the contraction multiplies with both projections
-    auto is_gu = [&](int kb) { return MODE == GLU_FORWARD || (MODE == GLU_BACKWARD && kb >= p.blocks0); };
+    auto is_gu = [&](int kb) { return MODE == GLU_FORWARD || (MODE == GLU_BACKWARD && kb >= p.q[0].blocks0); };
 
     if (warp == EPILOGUE_WARPS + 1) {
         // ---- copies ----
@@ -342,11 +367,12 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             };
             for (long long t = first_tile; t < tiles && ok; t += stride) {
                 const Tile x = tile_of(p, t);
+                const Problem &q = p.q[x.q];
                 const int m0 = (PAIR ? 2 * x.m + (int)rank : x.m) * TM, n0 = x.n * TN;
                 for (int kb = x.k_lo; kb < x.k_hi; ++kb) {
                     ok = mbar_wait(empty(s), phase, gave_up);
                     if (!ok) break;
-                    const int part = kb >= p.blocks0, k = (part ? kb - p.blocks0 : kb) * TK;
+                    const int part = kb >= q.blocks0, k = (part ? kb - q.blocks0 : kb) * TK;
                     const bool gu = is_gu(kb);
                     const uint32_t at = base + s * S::STAGE, bt = at + NP * S::A_PIECE;
                     const uint32_t bar = PAIR ? mapa(full(s), 0) : full(s);
@@ -354,17 +380,17 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                         mbar_expect(full(s), (uint32_t)((PAIR ? 2 : 1) * NP * (S::A_PIECE + (gu ? S::ROWS_GU : S::ROWS_ONE) * TK * 2)));
 #pragma unroll
                     for (int i = 0; i < NP; ++i) {
-                        operand(&p.a[part], p.a_across[part], at + i * S::A_PIECE, TM, m0, k, i, bar);
+                        operand(&q.a[part], q.a_across[part], at + i * S::A_PIECE, TM, m0, k, i, bar);
                         const uint32_t bi = bt + i * S::B_PIECE;
                         if (gu) {
                             if (PAIR) {
-                                operand(&p.b[1 + rank], false, bi, TN, n0, k, i, bar);
+                                operand(&q.b[1 + rank], false, bi, TN, n0, k, i, bar);
                             } else {
-                                operand(&p.b[1], false, bi, TN, n0, k, i, bar);
-                                operand(&p.b[2], false, bi + TN * TK * 2, TN, n0, k, i, bar);
+                                operand(&q.b[1], false, bi, TN, n0, k, i, bar);
+                                operand(&q.b[2], false, bi + TN * TK * 2, TN, n0, k, i, bar);
                             }
                         } else {
-                            operand(&p.b[part], p.b_across[part], bi, S::ROWS_ONE, n0 + (int)rank * S::ROWS_ONE, k, i, bar);
+                            operand(&q.b[part], q.b_across[part], bi, S::ROWS_ONE, n0 + (int)rank * S::ROWS_ONE, k, i, bar);
                         }
                     }
                     ++sent;
@@ -396,10 +422,11 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             bool ok = true;
             for (long long t = first_tile; t < tiles && ok; t += stride) {
                 const Tile x = tile_of(p, t);
+                const Problem &q = p.q[x.q];
                 for (int kb = x.k_lo; kb < x.k_hi; ++kb) {
-                    const int part = kb >= p.blocks0;
+                    const int part = kb >= q.blocks0;
                     const bool gu = is_gu(kb);
-                    const bool clear = NP > 1 || kb == x.k_lo || (MODE == GLU_BACKWARD && kb == p.blocks0);  // the first block of an accumulator
+                    const bool clear = NP > 1 || kb == x.k_lo || (MODE == GLU_BACKWARD && kb == q.blocks0);  // the first block of an accumulator
                     // (where the sets of dh lie behind a shared one, that of the tile before last has been taken: see the wait below)
                     if (clear && (!S::SHARED_SET || gu)) {
                         ok = mbar_wait(taken(b), set_phase, gave_up);
@@ -410,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (!ok) break;
                     fence_after();
                     const uint32_t d = tmem + (S::SHARED_SET ? (gu ? 0u : (2u + dh_set) * TN) : (uint32_t)(b * S::WIDTH));
-                    const bool aa = p.a_across[part], ba = !gu && p.b_across[part];
+                    const bool aa = q.a_across[part], ba = !gu && q.b_across[part];
                     const uint32_t idesc = (gu ? instr_desc<IM, MODE == LINEAR ? TN : 2 * TN, AB, false>() : instr_desc<IM, TN, AB, false>()) |
                                            (aa ? 1u << 15 : 0u) | (ba ? 1u << 16 : 0u);
                     // a step of 16 along the contraction: 32 bytes of a row, or 16 rows; panels of 64 across it lie 8 KB apart
@@ -459,8 +486,6 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         const int first = (warp >> 2) * SHARE;
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21) + first;
         float *bias_16 = reinterpret_cast<float *>(smem + S::BIAS) + warp * 32;
-        const void *bias_a = MODE == LINEAR ? p.bias : p.bias_gate, *bias_b = MODE == LINEAR ? nullptr : p.bias_up;
-        const bool biased = bias_a != nullptr || bias_b != nullptr;
         auto give_back = [&](int b) {
             fence_before();
             __syncwarp();
@@ -474,11 +499,24 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
         bool ok = true;
         for (long long t = first_tile; t < tiles && ok; t += stride) {
             const Tile x = tile_of(p, t);
+            const Problem &q = p.q[x.q];
+            const void *bias_a = MODE == LINEAR ? q.bias : p.bias_gate, *bias_b = MODE == LINEAR ? nullptr : p.bias_up;
+            const bool biased = bias_a != nullptr || bias_b != nullptr;
+            const bool split = MODE == LINEAR && q.splits > 1;
+            // a warp's part of a tile's shares: 16 columns of a lane's row as four vectors, lanes as neighbours
+            const long long mine = ((long long)x.m * q.n_tiles + x.n) * (PAIR ? 2 : 1) + rank;
+            float4 *shares = reinterpret_cast<float4 *>(q.partial) + ((mine * q.splits * EPILOGUE_WARPS + warp) * CHUNKS * 4) * 32 + lane;
+            const long long per_share = (long long)EPILOGUE_WARPS * CHUNKS * 4 * 32;
+            auto put_share = [&](int c, const float (&v)[16]) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    __stcg(shares + x.split * per_share + (c * 4 + i) * 32, make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+            };
             const long long row = ((long long)(PAIR ? 2 * x.m + rank : x.m)) * TM + (warp & 3) * 32 + lane;
             const int col = x.n * TN + first;
             float bias[CHUNKS];
 #pragma unroll
-            for (int c = 0; c < CHUNKS; ++c) bias[c] = biased ? lane_bias<T>(bias_a, bias_b, col + c * 16, p.N, lane) : 0.f;
+            for (int c = 0; c < CHUNKS; ++c) bias[c] = biased ? lane_bias<T>(bias_a, bias_b, col + c * 16, q.N, lane) : 0.f;
             auto place_bias = [&](int c) -> const float * {
                 if (!biased) return nullptr;
                 __syncwarp();
@@ -498,7 +536,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     // (dh is the third accumulator: two or three widths behind the first)
                     tmem_load_rows16<S::ACCS>(at, TN, v, S::SHARED_SET ? dh_set * TN : 0);
                     if (c == CHUNKS - 1) give_back(b);
-                    finish<T, MODE>(p, x.split, row, col + c * 16, place_bias(c), v);
+                    if (split) put_share(c, v[0]);
+                    else finish<T, MODE>(p, q, row, col + c * 16, place_bias(c), v);
                 }
                 if (++b == SETS) { b = 0; phase ^= 1u; }
                 dh_set ^= 1;
@@ -516,7 +555,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (!ok) break;
                     fence_after();
                     const uint32_t at = lanes + b * S::WIDTH;
-                    if (MODE == GLU_BACKWARD && kb < p.blocks0) {
+                    if (MODE == GLU_BACKWARD && kb < q.blocks0) {
 #pragma unroll
                         for (int c = 0; c < CHUNKS; ++c) {
                             float v[1][16];
@@ -541,7 +580,36 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c) finish<T, MODE>(p, x.split, row, col + c * 16, place_bias(c), sum[c]);
+                for (int c = 0; c < CHUNKS; ++c) {
+                    if (split) put_share(c, sum[c][0]);
+                    else finish<T, MODE>(p, q, row, col + c * 16, place_bias(c), sum[c]);
+                }
+            }
+            if constexpr (MODE == LINEAR) {
+                if (split) {  // the last share of this warp's part: all of them, in their order
+                    __threadfence();
+                    __syncwarp();
+                    unsigned before = 0u;
+                    if (lane == 0) before = atomicAdd(q.tickets + mine * EPILOGUE_WARPS + warp, 1u);
+                    if (__shfl_sync(FULL, before, 0) + 1u == (unsigned)q.splits) {
+                        __threadfence();
+#pragma unroll
+                        for (int c = 0; c < CHUNKS; ++c) {
+                            float v[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] = 0.f;
+#pragma unroll 2
+                            for (int s = 0; s < q.splits; ++s) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float4 w = __ldcg(shares + s * per_share + (c * 4 + i) * 32);
+                                    v[4 * i] += w.x; v[4 * i + 1] += w.y; v[4 * i + 2] += w.z; v[4 * i + 3] += w.w;
+                                }
+                            }
+                            finish_linear<T>(q, row, col + c * 16, place_bias(c), v);
+                        }
+                    }
+                }
             }
         }
     }
