@@ -137,12 +137,24 @@ __device__ __forceinline__ void sum_columns(const ColumnJob &job, int block)
     __syncthreads();
     if (!last) return;
     __threadfence();
+    // (each warp some of the shares, then the warps')
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const int at = group * 32 * VEC + e * 32 + lane;
+        float t = 0.f;
+        if (at < job.cols) {
+#pragma unroll 8
+            for (int s = warp; s < job.shares; s += 8) t += __ldcg(job.partial + (long long)s * job.cols + at);
+        }
+        part[warp][e * 32 + lane] = t;
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
         const int at = group * 32 * VEC + i;
-        if (at >= job.cols) continue;
         float t = 0.f;
-#pragma unroll 8
-        for (int s = 0; s < job.shares; ++s) t += __ldcg(job.partial + (long long)s * job.cols + at);
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += part[w][i];
+        if (at >= job.cols) continue;
         if (at < job.cols0) { if (job.out0 != nullptr) static_cast<T *>(job.out0)[at] = from_float<T>(t); }
         else if (at >= job.col1 && at < job.col1 + job.cols1) { if (job.out1 != nullptr) static_cast<T *>(job.out1)[at - job.col1] = from_float<T>(t); }
     }
@@ -276,7 +288,7 @@ Cut find_cut(const Size *sizes, int count)
 {
     // a block of the contraction of a 16-bit type: its products, or what L2 delivers; of float32: six products
     struct Kind { int tn; bool pair; double one, six; };
-    constexpr Kind kinds[] = {{256, true, 3.4, 12.5}, {128, true, 3.2, 8.0}, {128, false, 3.2, 9.0}, {64, false, 2.2, 5.0}};
+    constexpr Kind kinds[] = {{256, true, 3.4, 20.0}, {128, true, 3.2, 11.0}, {128, false, 3.2, 13.5}, {64, false, 2.2, 7.5}};
     constexpr bool wide = pieces_of<T> > 1;
     const double sms = sm_count();
     int most = 1;

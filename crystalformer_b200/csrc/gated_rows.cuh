@@ -58,25 +58,37 @@ __global__ void __launch_bounds__(THREADS) hidden_kernel(const __grid_constant__
 #pragma unroll
         for (int r = 0; r < R; ++r) g[j][r] = u[j][r] = 0.f;
     grid_dependency_wait();
-    for (int k = (in_group * 32 + lane) * VEC; k < D; k += warps * 32 * VEC) {
-        float a[UNITS][VEC], b[UNITS][VEC];
+    // two steps of weights on their way at a time
+    const int stride = warps * 32 * VEC;
+    for (int k = (in_group * 32 + lane) * VEC; k < D; k += 2 * stride) {
+        Raw<T, VEC> a[2][UNITS], b[2][UNITS];
 #pragma unroll
-        for (int j = 0; j < UNITS; ++j) {
-            const long long at = (long long)min(unit0 + j, F - 1) * D + k;
-            load_values<T, VEC>(wg + at, a[j]);
-            load_values<T, VEC>(wu + at, b[j]);
-        }
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float v[VEC];
-            load_values<T, VEC>(x + (long long)min(r, (int)d.N - 1) * d.ldx + k, v);
+            for (int j = 0; j < UNITS; ++j) {
+                const long long at = (long long)min(unit0 + j, F - 1) * D + k + t * stride;
+                a[t][j] = b[t][j] = Raw<T, VEC>{};
+                if (k + t * stride < D) { a[t][j] = load_raw<T, VEC>(wg + at); b[t][j] = load_raw<T, VEC>(wu + at); }
+            }
 #pragma unroll
-            for (int j = 0; j < UNITS; ++j)
+        for (int t = 0; t < 2; ++t) {
+            if (k + t * stride >= D) break;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    g[j][r] += a[j][e] * v[e];
-                    u[j][r] += b[j][e] * v[e];
+            for (int r = 0; r < R; ++r) {
+                float v[VEC];
+                load_values<T, VEC>(x + (long long)min(r, (int)d.N - 1) * d.ldx + k + t * stride, v);
+#pragma unroll
+                for (int j = 0; j < UNITS; ++j) {
+                    float wa[VEC], wb[VEC];
+                    expand<T, VEC>(a[t][j], wa);
+                    expand<T, VEC>(b[t][j], wb);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        g[j][r] += wa[e] * v[e];
+                        u[j][r] += wb[e] * v[e];
+                    }
                 }
+            }
         }
     }
 #pragma unroll
@@ -111,19 +123,37 @@ __global__ void __launch_bounds__(THREADS) output_kernel(const __grid_constant__
     for (int j = 0; j < UNITS; ++j)
 #pragma unroll
         for (int r = 0; r < R; ++r) s[j][r] = 0.f;
+    const int stride = warps * 32 * VEC, k0 = (in_group * 32 + lane) * VEC;
+    constexpr int AHEAD = 2;  // steps of weights on their way: the first ones from before the hidden units are there (they are the caller's)
+    Raw<T, VEC> a[AHEAD][UNITS];
+    auto fetch = [&](int t, int k) {
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j) {
+            a[t][j] = Raw<T, VEC>{};
+            if (k < F) a[t][j] = load_raw<T, VEC>(wd + (long long)min(unit0 + j, D - 1) * F + k);
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) fetch(t, k0 + t * stride);
     grid_dependency_wait();
-    for (int k = (in_group * 32 + lane) * VEC; k < F; k += warps * 32 * VEC) {
-        float a[UNITS][VEC];
+    for (int k = k0; k < F; k += AHEAD * stride) {
 #pragma unroll
-        for (int j = 0; j < UNITS; ++j) load_values<T, VEC>(wd + (long long)min(unit0 + j, D - 1) * F + k, a[j]);
+        for (int t = 0; t < AHEAD; ++t) {
+            const int at = k + t * stride;
+            if (at >= F) break;
+            float w[UNITS][VEC];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float v[VEC];
-            load_hidden<VEC>(h + (long long)min(r, (int)d.N - 1) * F + k, v);
+            for (int j = 0; j < UNITS; ++j) expand<T, VEC>(a[t][j], w[j]);
+            fetch(t, at + AHEAD * stride);
 #pragma unroll
-            for (int j = 0; j < UNITS; ++j)
+            for (int r = 0; r < R; ++r) {
+                float v[VEC];
+                load_hidden<VEC>(h + (long long)min(r, (int)d.N - 1) * F + at, v);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) s[j][r] += a[j][e] * v[e];
+                for (int j = 0; j < UNITS; ++j)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) s[j][r] += w[j][e] * v[e];
+            }
         }
     }
 #pragma unroll
@@ -148,18 +178,18 @@ __global__ void __launch_bounds__(THREADS) output_kernel(const __grid_constant__
 inline int warps_of(long long units, int per_group, long long steps)
 {
     int warps = 1;
-    while (warps < 8 && steps > warps && (units + per_group - 1) / per_group * warps < 16ll * sm_count()) warps *= 2;
+    while (warps < 8 && steps > warps && (units + per_group - 1) / per_group * warps < 24ll * sm_count()) warps *= 2;
     return warps;
 }
 
 template <class T, int VEC_X, int VEC_H, int R>
 int launch(const cf_gated_ffn &d, void *y, float *h, cudaStream_t s)
 {
-    constexpr int UNITS = 2;
-    const int hw = warps_of(d.F, UNITS, (d.D + 32 * VEC_X - 1) / (32 * VEC_X)), ow = warps_of(d.D, UNITS, (d.F + 32 * VEC_H - 1) / (32 * VEC_H));
-    const long long hg = (d.F + UNITS - 1) / UNITS, og = (d.D + UNITS - 1) / UNITS;
+    constexpr int UNITS = 2, OUT_UNITS = 4;  // (outputs: a block reads all of h, from L2)
+    const int hw = warps_of(d.F, UNITS, (d.D + 32 * VEC_X - 1) / (32 * VEC_X)), ow = warps_of(d.D, OUT_UNITS, (d.F + 32 * VEC_H - 1) / (32 * VEC_H));
+    const long long hg = (d.F + UNITS - 1) / UNITS, og = (d.D + OUT_UNITS - 1) / OUT_UNITS;
     hidden_kernel<T, VEC_X, R, UNITS><<<(unsigned)((hg * hw + 7) / 8), THREADS, 0, s>>>(d, h, hw);
-    launch_chained(output_kernel<T, VEC_H, R, UNITS>, dim3((unsigned)((og * ow + 7) / 8)), dim3(THREADS), 0, s, true, d, h, static_cast<T *>(y), ow);
+    launch_chained(output_kernel<T, VEC_H, R, OUT_UNITS>, dim3((unsigned)((og * ow + 7) / 8)), dim3(THREADS), 0, s, true, d, h, static_cast<T *>(y), ow);
     return launch_status("gated_rows");
 }
 

@@ -18,7 +18,9 @@
 // pieces (24 bits, any exponent), made once by a packing kernel or by the epilogue that produces it, and a product is six: piece 0
 // with 0, 1, 2, piece 1 with 0, 1 and piece 2 with 0 (what is left out is 2^-26 of a product).  The tensor core's running sums lose
 // low bits with every instruction, so that with three pieces each block of 64 has accumulators of its own, smallest products first,
-// and the sums over blocks are added in registers: errors are those of float32 sums (3e-7 relative at 512 terms).
+// and the sums over blocks are added in registers: errors are those of float32 sums (3e-7 relative at 512 terms).  The projections of
+// models of up to 128 features, two blocks, stay in their accumulators, the small products of both before the large ones: the
+// epilogue then takes a tile at once, beside the next one's products (backward of 133,120 rows, 128 x 512: 602 -> XXX us).
 //
 // All waits are bounded (tc5::mbar_wait); one that runs out ends the block after its copies and products in flight.
 #pragma once
@@ -82,6 +84,7 @@ struct Params {
     float *sums;              // or null: (32 rows each, 2 padded) sums of the columns of dg and du
 };
 constexpr int LINEAR_COUNT = 3;  // products that one launch may have
+constexpr int WHOLE = 2;
 template <int MODE> using ParamsOf = Params<MODE == LINEAR ? LINEAR_COUNT : 1>;
 
 template <class T, int MODE, int TN, bool PAIR>
@@ -94,14 +97,14 @@ struct Shape {
     static constexpr int STAGE = NP * (A_PIECE + B_PIECE);
     static constexpr int ROOM = 220 * 1024;
     static constexpr int STAGES = ROOM / STAGE < 8 ? ROOM / STAGE : 8;
-    static constexpr int WIDTH = MODE == LINEAR ? TN : 2 * TN;            // columns of what a product of one block fills at most
+    static constexpr int WIDTH = ACCS * TN;                               // columns of a set of accumulators: g, u, dh
     static constexpr bool SHARED_SET = NP == 1 && MODE == GLU_BACKWARD;   // one set, two of dh behind it
     static constexpr int SETS = SHARED_SET ? 1 : 2;
     static constexpr int USED = SHARED_SET ? 4 * TN : 2 * WIDTH;
     static constexpr int TMEM = USED <= 64 ? 64 : USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
     static constexpr int MISC = STAGES * STAGE, BIAS = MISC + 256;
     static constexpr int SMEM = BIAS + EPILOGUE_WARPS * 128;
-    static_assert(STAGES >= 2 && USED <= 512 && WIDTH <= 256, "tile");
+    static_assert(STAGES >= 2 && USED <= 512, "tile");
 };
 
 // ---- activations: value and derivative ---------------------------------------------------------------------------------------
@@ -345,6 +348,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
     }
     const long long first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, stride = PAIR ? gridDim.x >> 1 : gridDim.x;
     // whether a block of the contraction multiplies with both projections
+    // three pieces: whether an accumulator keeps the whole contraction (WHOLE blocks at most), or each block of it goes to registers
+    const bool whole = NP > 1 && MODE != LINEAR && p.q[0].blocks0 <= WHOLE;
     auto is_gu = [&](int kb) { return MODE == GLU_FORWARD || (MODE == GLU_BACKWARD && kb >= p.q[0].blocks0); };
 
     if (warp == EPILOGUE_WARPS + 1) {
@@ -426,9 +431,10 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 for (int kb = x.k_lo; kb < x.k_hi; ++kb) {
                     const int part = kb >= q.blocks0;
                     const bool gu = is_gu(kb);
-                    const bool clear = NP > 1 || kb == x.k_lo || (MODE == GLU_BACKWARD && kb == q.blocks0);  // the first block of an accumulator
+                    const bool starts = kb == x.k_lo || (MODE == GLU_BACKWARD && kb == q.blocks0);  // a part
+                    const bool clear = NP == 1 ? starts : !whole || starts;  // the first block of an accumulator
                     // (where the sets of dh lie behind a shared one, that of the tile before last has been taken: see the wait below)
-                    if (clear && (!S::SHARED_SET || gu)) {
+                    if (S::SHARED_SET ? clear && gu : NP > 1 && !whole ? true : kb == x.k_lo) {
                         ok = mbar_wait(taken(b), set_phase, gave_up);
                         if (!ok) break;
                         fence_after();
@@ -436,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     ok = mbar_wait(full(s), phase, gave_up);
                     if (!ok) break;
                     fence_after();
-                    const uint32_t d = tmem + (S::SHARED_SET ? (gu ? 0u : (2u + dh_set) * TN) : (uint32_t)(b * S::WIDTH));
+                    const uint32_t d = tmem + (S::SHARED_SET ? (gu ? 0u : (2u + dh_set) * TN) : (uint32_t)(b * S::WIDTH + (MODE == GLU_BACKWARD && !gu ? 2 * TN : 0)));
                     const bool aa = q.a_across[part], ba = !gu && q.b_across[part];
                     const uint32_t idesc = (gu ? instr_desc<IM, MODE == LINEAR ? TN : 2 * TN, AB, false>() : instr_desc<IM, TN, AB, false>()) |
                                            (aa ? 1u << 15 : 0u) | (ba ? 1u << 16 : 0u);
@@ -449,25 +455,49 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 #pragma unroll
                         for (int ks = 0; ks < TK / 16; ++ks) mma(d, a0 + ks * a_step, b0 + ks * b_step, idesc, !(clear && ks == 0));
                     } else {
+                        // small products first; of a whole contraction those of both blocks, before the large ones of either
+                        auto small = [&](uint64_t ak0, uint64_t bk0, bool first) {
 #pragma unroll
-                        for (int ks = 0; ks < TK / 16; ++ks) {
-                            const uint64_t ak = a0 + ks * a_step, bk = b0 + ks * b_step;
-                            mma(d, ak + 2 * AP, bk, idesc, ks > 0);
-                            mma(d, ak, bk + 2 * BP, idesc, true);
-                            mma(d, ak + AP, bk + BP, idesc, true);
+                            for (int ks = 0; ks < TK / 16; ++ks) {
+                                const uint64_t ak = ak0 + ks * a_step, bk = bk0 + ks * b_step;
+                                mma(d, ak + 2 * AP, bk, idesc, !(first && ks == 0));
+                                mma(d, ak, bk + 2 * BP, idesc, true);
+                                mma(d, ak + AP, bk + BP, idesc, true);
+                            }
+#pragma unroll
+                            for (int ks = 0; ks < TK / 16; ++ks) {
+                                const uint64_t ak = ak0 + ks * a_step, bk = bk0 + ks * b_step;
+                                mma(d, ak + AP, bk, idesc, true);
+                                mma(d, ak, bk + BP, idesc, true);
+                            }
+                        };
+                        auto large = [&](uint64_t ak0, uint64_t bk0) {
+#pragma unroll
+                            for (int ks = 0; ks < TK / 16; ++ks) mma(d, ak0 + ks * a_step, bk0 + ks * b_step, idesc, true);
+                        };
+                        small(a0, b0, clear);
+                        if (whole && starts && q.blocks0 == 2) {
+                            int s2 = s + 1;
+                            uint32_t phase2 = phase;
+                            if (s2 == STAGES) { s2 = 0; phase2 ^= 1u; }
+                            ok = mbar_wait(full(s2), phase2, gave_up);
+                            if (!ok) break;
+                            fence_after();
+                            const uint64_t a1 = smem_desc(base + s2 * S::STAGE, 8192, 1024), b1 = smem_desc(base + s2 * S::STAGE + NP * S::A_PIECE, 8192, 1024);
+                            small(a1, b1, false);
+                            large(a0, b0);
+                            commit(empty(s));
+                            large(a1, b1);
+                            s = s2;
+                            phase = phase2;
+                            ++kb;
+                        } else {
+                            large(a0, b0);
                         }
-#pragma unroll
-                        for (int ks = 0; ks < TK / 16; ++ks) {
-                            const uint64_t ak = a0 + ks * a_step, bk = b0 + ks * b_step;
-                            mma(d, ak + AP, bk, idesc, true);
-                            mma(d, ak, bk + BP, idesc, true);
-                        }
-#pragma unroll
-                        for (int ks = 0; ks < TK / 16; ++ks) mma(d, a0 + ks * a_step, b0 + ks * b_step, idesc, true);
                     }
                     commit(empty(s));
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
-                    if (NP > 1 || kb == x.k_hi - 1) {
+                    if ((NP > 1 && !whole) || kb == x.k_hi - 1) {
                         commit(ready(b));
                         if (++b == SETS) { b = 0; set_phase ^= 1u; }
                     }
@@ -524,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 __syncwarp();
                 return bias_16;
             };
-            if constexpr (NP == 1) {
+            if (NP == 1 || whole) {
                 ok = mbar_wait(ready(b), phase, gave_up);
                 ok = __all_sync(FULL, ok);
                 if (!ok) break;
@@ -541,7 +571,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 }
                 if (++b == SETS) { b = 0; phase ^= 1u; }
                 dh_set ^= 1;
-            } else {
+            } else if constexpr (NP > 1) {
                 float sum[CHUNKS][S::ACCS][16];
 #pragma unroll
                 for (int c = 0; c < CHUNKS; ++c)
@@ -559,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
 #pragma unroll
                         for (int c = 0; c < CHUNKS; ++c) {
                             float v[1][16];
-                            tmem_load_rows16<1>(at + c * 16, TN, v, 0);
+                            tmem_load_rows16<1>(at + 2 * TN + c * 16, TN, v, 0);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) sum[c][S::ACCS - 1][i] += v[0][i];
                         }
