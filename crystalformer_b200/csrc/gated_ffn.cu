@@ -30,7 +30,7 @@ struct PackJob {
     long long groups;  // of eight values, with those that pad a row
     bool transposed;   // rows and cols are those of the planes, the source's the other way round
 };
-constexpr int PACK_JOBS = 5, COLUMN_SHARES = 256;
+constexpr int PACK_JOBS = 5, COLUMN_SHARES = 512;
 struct PackJobs {
     PackJob j[PACK_JOBS];
 };
@@ -113,7 +113,7 @@ __device__ __forceinline__ void sum_columns(const ColumnJob &job, int block)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) sum[e] = low[e] = 0.f;
     if (col < job.cols) {
-#pragma unroll 4
+#pragma unroll 8
         for (long long n = lo + warp; n < hi; n += 8) {
             float v[VEC];
             load_values<X, VEC>(x + n * job.cols + col, v);
@@ -164,9 +164,9 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const __grid_constant__
 {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int first = jobs.j[0].groups * jobs.j[0].shares;
-    if ((int)blockIdx.x < first) sum_columns<T, float, 4>(jobs.j[0], blockIdx.x);
-    else sum_columns<T, T, VEC>(jobs.j[1], blockIdx.x - first);
+    const int first = jobs.j[1].groups * jobs.j[1].shares;  // (the longer shares first)
+    if ((int)blockIdx.x < first) sum_columns<T, T, VEC>(jobs.j[1], blockIdx.x);
+    else sum_columns<T, float, 4>(jobs.j[0], blockIdx.x - first);
 }
 
 // ---- tensor maps ----------------------------------------------------------------------------------------------------------------------
@@ -265,6 +265,7 @@ struct Linear {
     int N;
     void *out0, *out1;
     long long rows0, row1, rows1, ld_out;
+    bool transposed;
     const void *bias;
     int splits;
 };
@@ -377,6 +378,7 @@ int run_linear(const Linear *products, int count, const Cut &cut, float *partial
         CF_REQUIRE(q.tiles < (1ll << 31), CF_ERR_RANGE, "cf_gated_ffn: %lld tiles", q.tiles);
         q.out0 = l.out0; q.out1 = l.out1;
         q.rows0 = l.rows0; q.row1 = l.row1; q.rows1 = l.rows1; q.ld_out = l.ld_out;
+        q.transposed = l.transposed;
         q.bias = l.bias;
         if (q.splits > 1) {
             q.partial = partial;
@@ -437,7 +439,7 @@ struct Plan {
             dg = {{g, 2 * Fp, d.N * 2 * Fp}, d.N, d.F};
             du = {{g ? g + Fp : g, 2 * Fp, d.N * 2 * Fp}, d.N, d.F};
             const int rows = blocks_of(d.N);  // (a call that leaves a gradient out cuts the others the same way)
-            const Size every[3] = {{d.N, (int)d.D, 2 * blocks_of(d.F)}, {2 * Fp, (int)d.D, rows}, {d.D, (int)d.F, rows}};
+            const Size every[3] = {{d.N, (int)d.D, 2 * blocks_of(d.F)}, {2 * Fp, (int)d.D, rows}, {d.F, (int)d.D, rows}};
             cut = linear_cut<T>(every, 3);
             sums = c.take<float>((size_t)((d.N + 31) / 32) * 2 * Fp);
             column_shares = c.take<float>((size_t)COLUMN_SHARES * (2 * Fp + d.D));
@@ -542,7 +544,7 @@ int run_columns(const Plan<T> &plan, const cf_gated_ffn_grads &g, cudaStream_t s
         j.x = x; j.rows = rows; j.cols = cols;
         j.groups = (cols + 32 * vec - 1) / (32 * vec);
         // (enough blocks to fill the GPU, of 32 rows at least, few enough for the last one to add up)
-        j.shares = (int)std::max(1ll, std::min<long long>({(long long)COLUMN_SHARES, rows / 32, std::max(1ll, 6ll * sm_count() / j.groups)}));
+        j.shares = (int)std::max(1ll, std::min<long long>({(long long)COLUMN_SHARES, rows / 32, std::max(1ll, 3ll * sm_count() / j.groups)}));
         j.partial = partial; j.tickets = tickets;
     };
     unsigned *tickets = plan.tickets + plan.cut.tickets;
@@ -600,12 +602,14 @@ int backward(const cf_gated_ffn &d, const cf_gated_ffn_grads &g, void *workspace
     }
     if (g.w_down) {
         Linear &l = products[count++];
-        l.a[0] = plan.gy; l.b[0] = plan.h;
+        // h^T gy, stored transposed: F is the larger side as a rule, and tiles are taller than they are wide
+        l.a[0] = plan.h; l.b[0] = plan.gy;
         l.a_across[0] = l.b_across[0] = true;
         l.parts = 1;
         l.K[0] = d.N;
-        l.M = D; l.N = F;
-        l.out0 = g.w_down; l.rows0 = D; l.row1 = D; l.ld_out = F;
+        l.M = F; l.N = D;
+        l.out0 = g.w_down; l.rows0 = F; l.row1 = F; l.ld_out = F;
+        l.transposed = true;
         l.splits = plan.cut.splits[2];
     }
     if ((rc = run_linear<T>(products, count, plan.cut, plan.partial, plan.tickets, s)) != CF_OK) return rc;

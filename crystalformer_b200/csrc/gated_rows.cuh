@@ -1,7 +1,13 @@
 // The gated feed-forward of a few rows: the three weights are read once, which is all the time that it needs (at the largest sizes of
-// a GPU's memory bandwidth, at the smallest of two launches in a chain).  A group of WARPS warps computes UNITS neighbouring hidden
-// units (then outputs) of all rows: lanes walk the contraction, eight or four weights of each unit at a time, with the rows' values
-// from L1.  h stays float32 between the two kernels.
+// a GPU's memory bandwidth, at the smallest of two launches in a chain).
+//
+// float32, and values that do not lie on 16 bytes: a group of `warps` warps computes UNITS neighbouring hidden units (then outputs) of
+// all rows; lanes walk the contraction, four weights of each unit at a time, with the rows' values from L1.
+//
+// 16-bit types: multiplying and adding in float32 would take longer than the weights need to come (31 us for four rows of 2048 x 5632,
+// whose 69 MB come in 10.6), so products are taken by mma.sync m16n8k16: 16 units by up to eight rows.  The sum does not mind which
+// k an operand calls its own: lane t of a group of four takes eight neighbours, k = 8 t .. 8 t + 7 of each 32, of its two units and of
+// its row, in one 16-byte load each, and both operands of two products are there.  A block's warps share the contraction.
 #pragma once
 #include "common.cuh"
 #include "tile_gemm.cuh"
@@ -58,37 +64,25 @@ __global__ void __launch_bounds__(THREADS) hidden_kernel(const __grid_constant__
 #pragma unroll
         for (int r = 0; r < R; ++r) g[j][r] = u[j][r] = 0.f;
     grid_dependency_wait();
-    // two steps of weights on their way at a time
-    const int stride = warps * 32 * VEC;
-    for (int k = (in_group * 32 + lane) * VEC; k < D; k += 2 * stride) {
-        Raw<T, VEC> a[2][UNITS], b[2][UNITS];
+    for (int k = (in_group * 32 + lane) * VEC; k < D; k += warps * 32 * VEC) {
+        float a[UNITS][VEC], b[UNITS][VEC];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int j = 0; j < UNITS; ++j) {
+            const long long at = (long long)min(unit0 + j, F - 1) * D + k;
+            load_values<T, VEC>(wg + at, a[j]);
+            load_values<T, VEC>(wu + at, b[j]);
+        }
 #pragma unroll
-            for (int j = 0; j < UNITS; ++j) {
-                const long long at = (long long)min(unit0 + j, F - 1) * D + k + t * stride;
-                a[t][j] = b[t][j] = Raw<T, VEC>{};
-                if (k + t * stride < D) { a[t][j] = load_raw<T, VEC>(wg + at); b[t][j] = load_raw<T, VEC>(wu + at); }
-            }
+        for (int r = 0; r < R; ++r) {
+            float v[VEC];
+            load_values<T, VEC>(x + (long long)min(r, (int)d.N - 1) * d.ldx + k, v);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            if (k + t * stride >= D) break;
+            for (int j = 0; j < UNITS; ++j)
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float v[VEC];
-                load_values<T, VEC>(x + (long long)min(r, (int)d.N - 1) * d.ldx + k + t * stride, v);
-#pragma unroll
-                for (int j = 0; j < UNITS; ++j) {
-                    float wa[VEC], wb[VEC];
-                    expand<T, VEC>(a[t][j], wa);
-                    expand<T, VEC>(b[t][j], wb);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        g[j][r] += wa[e] * v[e];
-                        u[j][r] += wb[e] * v[e];
-                    }
+                for (int e = 0; e < VEC; ++e) {
+                    g[j][r] += a[j][e] * v[e];
+                    u[j][r] += b[j][e] * v[e];
                 }
-            }
         }
     }
 #pragma unroll
@@ -178,8 +172,129 @@ __global__ void __launch_bounds__(THREADS) output_kernel(const __grid_constant__
 inline int warps_of(long long units, int per_group, long long steps)
 {
     int warps = 1;
-    while (warps < 8 && steps > warps && (units + per_group - 1) / per_group * warps < 24ll * sm_count()) warps *= 2;
+    while (warps < 8 && steps > warps && (units + per_group - 1) / per_group * warps < 16ll * sm_count()) warps *= 2;
     return warps;
+}
+
+// ---- 16-bit types, on 16 bytes --------------------------------------------------------------------------------------------------
+template <class T>
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 32 of the contraction: eight of them of units g and g + 8 (lo, hi) and of row g
+template <class T>
+__device__ __forceinline__ void mma_32(float (&c)[4], const uint4 &lo, const uint4 &hi, const uint4 &x)
+{
+    mma_16x8x16<T>(c, lo.x, hi.x, lo.y, hi.y, x.x, x.y);
+    mma_16x8x16<T>(c, lo.z, hi.z, lo.w, hi.w, x.z, x.w);
+}
+
+constexpr int MMA_AHEAD = 4;  // steps of 32 on their way
+
+// MATS matrices of (M, K) weights by up to eight rows x (ld) of K values: sums[mat][unit of 16][row of 8] of the block's 16 units in
+// `part`, (warps, MATS, 16, 8).  `wait`: x comes from the kernel before (the weights are the caller's, and may be fetched earlier).
+template <class T, int MATS, bool WAIT>
+__device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int K, const T *x, long long ld, int rows, int unit0, int warps, float *part)
+{
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const long long lo = (long long)min(unit0 + g, M - 1) * K + 8 * t, hi = (long long)min(unit0 + g + 8, M - 1) * K + 8 * t;
+    const T *xr = x + (long long)min(g, rows - 1) * ld + 8 * t;
+    uint4 a[MMA_AHEAD][MATS][2];
+    auto fetch = [&](int i, int k) {
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+            a[i][m][0] = a[i][m][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (k + 8 * t < K) {
+                a[i][m][0] = __ldg(reinterpret_cast<const uint4 *>(w[m] + lo + k));
+                a[i][m][1] = __ldg(reinterpret_cast<const uint4 *>(w[m] + hi + k));
+            }
+        }
+    };
+    const int k0 = warp * 32, step = warps * 32;
+#pragma unroll
+    for (int i = 0; i < MMA_AHEAD; ++i) fetch(i, k0 + i * step);
+    if constexpr (WAIT) grid_dependency_wait();
+    float c[MATS][4];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[m][i] = 0.f;
+    for (int k = k0; k < K; k += MMA_AHEAD * step) {
+        uint4 b[MMA_AHEAD];
+#pragma unroll
+        for (int i = 0; i < MMA_AHEAD; ++i) {
+            const int at = k + i * step;
+            b[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (at + 8 * t < K && g < rows) b[i] = *reinterpret_cast<const uint4 *>(xr + at);
+        }
+#pragma unroll
+        for (int i = 0; i < MMA_AHEAD; ++i) {
+            const int at = k + i * step;
+            if (at >= K) break;
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) mma_32<T>(c[m], a[i][m][0], a[i][m][1], b[i]);
+            fetch(i, at + MMA_AHEAD * step);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) {
+        float *to = part + ((warp * MATS + m) * 16 + g) * 8 + 2 * t;
+        to[0] = c[m][0]; to[1] = c[m][1];
+        to[64] = c[m][2]; to[65] = c[m][3];
+    }
+    __syncthreads();
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) hidden_mma_kernel(const __grid_constant__ cf_gated_ffn d, T *h)
+{
+    __shared__ float part[8 * 2 * 128];
+    grid_launch_dependents();
+    const int unit0 = blockIdx.x * 16, F = (int)d.F, N = (int)d.N;
+    const T *const w[2] = {static_cast<const T *>(d.w_gate), static_cast<const T *>(d.w_up)};
+    weigh_rows<T, 2, false>(w, F, (int)d.D, static_cast<const T *>(d.x), d.ldx, N, unit0, 8, part);
+    const int f = unit0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
+    if (r >= N || f >= F) return;
+    float a = 0.f, b = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a += part[(i * 2 * 16 + (threadIdx.x & 15)) * 8 + r];
+        b += part[((i * 2 + 1) * 16 + (threadIdx.x & 15)) * 8 + r];
+    }
+    if (d.b_gate) a += to_float(static_cast<const T *>(d.b_gate)[f]);
+    if (d.b_up) b += to_float(static_cast<const T *>(d.b_up)[f]);
+    h[(long long)r * F + f] = from_float<T>(activation(d.activation, a) * b);
+}
+
+template <class T>
+__global__ void __launch_bounds__(512) output_mma_kernel(const __grid_constant__ cf_gated_ffn d, const T *h, T *y)
+{
+    __shared__ float part[16 * 128];
+    grid_launch_dependents();
+    const int unit0 = blockIdx.x * 16, D = (int)d.D, N = (int)d.N;
+    const T *const w[1] = {static_cast<const T *>(d.w_down)};
+    weigh_rows<T, 1, true>(w, D, (int)d.F, h, d.F, N, unit0, 16, part);
+    const int c = unit0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
+    if (r >= N || c >= D) return;
+    float a = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a += part[(i * 16 + (threadIdx.x & 15)) * 8 + r];
+    if (d.b_down) a += to_float(static_cast<const T *>(d.b_down)[c]);
+    y[(long long)r * D + c] = from_float<T>(a);
+}
+
+template <class T>
+int launch_mma(const cf_gated_ffn &d, void *y, T *h, cudaStream_t s)
+{
+    hidden_mma_kernel<T><<<(unsigned)((d.F + 15) / 16), 256, 0, s>>>(d, h);
+    launch_chained(output_mma_kernel<T>, dim3((unsigned)((d.D + 15) / 16)), dim3(512), 0, s, true, d, static_cast<const T *>(h), static_cast<T *>(y));
+    return launch_status("gated_rows");
 }
 
 template <class T, int VEC_X, int VEC_H, int R>
@@ -195,16 +310,19 @@ int launch(const cf_gated_ffn &d, void *y, float *h, cudaStream_t s)
 
 }  // namespace rows
 
-// y of up to GATED_ROWS rows; h: N F floats.
+// y of up to GATED_ROWS rows; h: N F floats (or, by mma.sync, values of the type: rounded once, as by the tiles).
 template <class T>
 int gated_rows(const cf_gated_ffn &d, void *y, float *h, cudaStream_t s)
 {
     constexpr int V = 16 / sizeof(T);
     const bool wide = d.D % V == 0 && d.F % V == 0 && d.ldx % V == 0 && aligned_to(d.x, 16) && aligned_to(d.w_gate, 16) && aligned_to(d.w_up, 16) &&
                       aligned_to(d.w_down, 16);
+    if constexpr (sizeof(T) == 2) {
+        if (wide) return rows::launch_mma<T>(d, y, reinterpret_cast<T *>(h), s);
+    }
     auto go = [&](auto rows) {
         constexpr int R = decltype(rows)::value;
-        return wide ? rows::launch<T, V, V, R>(d, y, h, s) : rows::launch<T, 1, 1, R>(d, y, h, s);
+        return sizeof(T) == 4 && wide ? rows::launch<T, sizeof(T) == 4 ? 4 : 1, sizeof(T) == 4 ? 4 : 1, R>(d, y, h, s) : rows::launch<T, 1, 1, R>(d, y, h, s);
     };
     if (d.N <= 1) return go(std::integral_constant<int, 1>());
     if (d.N <= 2) return go(std::integral_constant<int, 2>());

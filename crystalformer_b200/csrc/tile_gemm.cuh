@@ -20,7 +20,7 @@
 // low bits with every instruction, so that with three pieces each block of 64 has accumulators of its own, smallest products first,
 // and the sums over blocks are added in registers: errors are those of float32 sums (3e-7 relative at 512 terms).  The projections of
 // models of up to 128 features, two blocks, stay in their accumulators, the small products of both before the large ones: the
-// epilogue then takes a tile at once, beside the next one's products (backward of 133,120 rows, 128 x 512: 602 -> XXX us).
+// epilogue then takes a tile at once, beside the next one's products (backward of 133,120 rows, 128 x 512: 602 -> 455 us).
 //
 // All waits are bounded (tc5::mbar_wait); one that runs out ends the block after its copies and products in flight.
 #pragma once
@@ -63,6 +63,7 @@ struct Problem {
     // LINEAR: rows [0, rows0) to out0, rows [row1, row1 + rows1) to out1
     void *out0, *out1;
     long long rows0, row1, rows1, ld_out;
+    int transposed;           // out0 (N, rows0): its rows are the columns
     const void *bias;
     // splits > 1: every share of a tile, and how many of a warp's part of it are there (zero before); who brings the last adds them
     float *partial;
@@ -262,6 +263,13 @@ __device__ __forceinline__ void finish_linear(const Problem &q, long long row, i
     if (row >= q.M || col >= q.N) return;
     if (bias != nullptr) add_16(bias, v);
     T *to;
+    if (q.transposed) {  // (a warp's 32 rows are neighbours there)
+        to = static_cast<T *>(q.out0) + (long long)col * q.ld_out + row;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (col + i < q.N) to[i * q.ld_out] = from_float<T>(v[i]);
+        return;
+    }
     if (row < q.rows0) to = static_cast<T *>(q.out0) + row * q.ld_out;
     else if (row >= q.row1 && row < q.row1 + q.rows1) to = static_cast<T *>(q.out1) + (row - q.row1) * q.ld_out;
     else return;
