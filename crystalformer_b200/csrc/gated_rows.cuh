@@ -195,11 +195,9 @@ __device__ __forceinline__ void mma_32(float (&c)[4], const uint4 &lo, const uin
     mma_16x8x16<T>(c, lo.z, hi.z, lo.w, hi.w, x.z, x.w);
 }
 
-constexpr int MMA_AHEAD = 4;  // steps of 32 on their way
-
 // MATS matrices of (M, K) weights by up to eight rows x (ld) of K values: sums[mat][unit of 16][row of 8] of the block's 16 units in
-// `part`, (warps, MATS, 16, 8).  `wait`: x comes from the kernel before (the weights are the caller's, and may be fetched earlier).
-template <class T, int MATS, bool WAIT>
+// `part`, (warps, MATS, 16, 8).  MMA_AHEAD: steps of 32 on their way.  `wait`: x comes from the kernel before (the weights are the caller's, and may be fetched earlier).
+template <class T, int MATS, int MMA_AHEAD, bool WAIT>
 __device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int K, const T *x, long long ld, int rows, int unit0, int warps, float *part)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -252,13 +250,13 @@ __device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) hidden_mma_kernel(const __grid_constant__ cf_gated_ffn d, T *h)
+__global__ void __launch_bounds__(256, 3) hidden_mma_kernel(const __grid_constant__ cf_gated_ffn d, T *h)
 {
     __shared__ float part[8 * 2 * 128];
     grid_launch_dependents();
     const int unit0 = blockIdx.x * 16, F = (int)d.F, N = (int)d.N;
     const T *const w[2] = {static_cast<const T *>(d.w_gate), static_cast<const T *>(d.w_up)};
-    weigh_rows<T, 2, false>(w, F, (int)d.D, static_cast<const T *>(d.x), d.ldx, N, unit0, 8, part);
+    weigh_rows<T, 2, 3, false>(w, F, (int)d.D, static_cast<const T *>(d.x), d.ldx, N, unit0, 8, part);
     const int f = unit0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
     if (r >= N || f >= F) return;
     float a = 0.f, b = 0.f;
@@ -279,7 +277,7 @@ __global__ void __launch_bounds__(512) output_mma_kernel(const __grid_constant__
     grid_launch_dependents();
     const int unit0 = blockIdx.x * 16, D = (int)d.D, N = (int)d.N;
     const T *const w[1] = {static_cast<const T *>(d.w_down)};
-    weigh_rows<T, 1, true>(w, D, (int)d.F, h, d.F, N, unit0, 16, part);
+    weigh_rows<T, 1, 6, true>(w, D, (int)d.F, h, d.F, N, unit0, 16, part);
     const int c = unit0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
     if (r >= N || c >= D) return;
     float a = 0.f;
