@@ -137,17 +137,26 @@ __device__ __forceinline__ void sum_columns(const ColumnJob &job, int block)
     __syncthreads();
     if (!last) return;
     __threadfence();
-    // (each warp some of the shares, then the warps')
+    // (each warp some of the shares, a lane VEC columns as before, then the warps')
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        const int at = group * 32 * VEC + e * 32 + lane;
-        float t = 0.f;
-        if (at < job.cols) {
+    for (int e = 0; e < VEC; ++e) sum[e] = 0.f;
+    if (col < job.cols) {
 #pragma unroll 8
-            for (int s = warp; s < job.shares; s += 8) t += __ldcg(job.partial + (long long)s * job.cols + at);
+        for (int s = warp; s < job.shares; s += 8) {
+            const float *from = job.partial + (long long)s * job.cols + col;
+            if constexpr (VEC == 1) {
+                sum[0] += __ldcg(from);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(from + e));
+                    sum[e] += v.x; sum[e + 1] += v.y; sum[e + 2] += v.z; sum[e + 3] += v.w;
+                }
+            }
         }
-        part[warp][e * 32 + lane] = t;
     }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) part[warp][lane * VEC + e] = sum[e];
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
         const int at = group * 32 * VEC + i;
@@ -544,7 +553,7 @@ int run_columns(const Plan<T> &plan, const cf_gated_ffn_grads &g, cudaStream_t s
         j.x = x; j.rows = rows; j.cols = cols;
         j.groups = (cols + 32 * vec - 1) / (32 * vec);
         // (enough blocks to fill the GPU, of 32 rows at least, few enough for the last one to add up)
-        j.shares = (int)std::max(1ll, std::min<long long>({(long long)COLUMN_SHARES, rows / 32, std::max(1ll, 3ll * sm_count() / j.groups)}));
+        j.shares = (int)std::max(1ll, std::min<long long>({(long long)COLUMN_SHARES, rows / 32, std::max(1ll, 2ll * sm_count() / j.groups)}));
         j.partial = partial; j.tickets = tickets;
     };
     unsigned *tickets = plan.tickets + plan.cut.tickets;
