@@ -5,15 +5,18 @@
 //   what lies behind the 2 P rotated entries of a head passes with its norm alone.
 //   backward, g' = the output's gradient turned back:  gw_d = sum g'_d x_d r,  gx_d = r (w_d g'_d - x_d r^2 mean_d'(w g' x)).
 //
-// Bound by memory (2 + 2 bytes or 4 + 4 a value forward), as long as the sines do not dominate: an angle is computed once per key
-// head and used for that key head and the query heads that share it.  A head is held by the fewest lanes (a power of two) that
-// take it in slots of 2 VEC values - a pair of vectors whose entries are partners - so that sums of squares are a few shuffles and
-// nothing is exchanged for the rotation.  A group of lanes walks the rows with the same heads of each; the next head's values are
-// on their way while one is computed (without that, and with 16-byte vectors' twice as
-// many registers, the backward of 16,384 rows of 32 + 8 heads of 128 took 353 us).  Waves count cycles per unit of position: the
-// products are exact (a rounded product and its fused remainder), whole turns are dropped before the parts are added, and an angle
-// is off by 2^-24 turns out to 2^24 turns of an axis; whole-numbered waves on fractional coordinates thus do not see lattice
-// translations at all.
+// What a pass cannot do without is memory traffic (2 + 2 bytes or 4 + 4 a value forward), but heads are short and 16-bit values many:
+// instruction issue (65 to 70 % of the slots at two blocks per SM) binds it first.  So: an angle is computed once per key head and used
+// for that key head and the query heads that share it.  A head is held by the fewest lanes (a power of two) that take it in slots of
+// 2 VEC values - a pair of vectors whose entries are partners - so that sums of squares are a few shuffles and nothing is exchanged for
+// the rotation.  A group of lanes walks the rows with the same heads of each: its weights stay in registers, and the next head's values
+// are on their way while one is computed.  Key and query heads are separate code (with one loop over both, selects and predicates
+// took half of the instructions: backward of 16,384 rows of 32 + 8 heads of 128, bfloat16, 167 us against 138).  16-byte vectors
+// forward (72 us there, 101 with 8 bytes); backward 8 bytes, since 16 would need more registers than two blocks on an SM leave.
+// Waves count cycles per unit of position: the products are exact (a rounded product and its fused remainder), whole turns are
+// dropped before the parts are added, and an angle is off by 2^-24 turns out to 2^24 turns of an axis; whole-numbered waves on
+// fractional coordinates thus do not see lattice translations at all.  133,120 rows of 8 + 8 heads of 16, float32, waves of each head:
+// 65 us forward (4.2 TB/s), 91 us backward (4.5 TB/s).
 //
 // The weights' gradients are sums over all rows: each lane keeps its entries' in registers, a block adds its lanes' in a fixed order,
 // and a second kernel adds the blocks'.
@@ -52,40 +55,44 @@ __device__ __forceinline__ Place place_of(const HeadArgs &p, int slot)
 
 __device__ __forceinline__ float lanes_sum(float v, int lanes)
 {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    if (lanes > 1) v += __shfl_xor_sync(FULL, v, 1);
+    if (lanes > 2) v += __shfl_xor_sync(FULL, v, 2);
+    if (lanes > 4) v += __shfl_xor_sync(FULL, v, 4);
+    if (lanes > 8) v += __shfl_xor_sync(FULL, v, 8);
+    if (lanes > 16) v += __shfl_xor_sync(FULL, v, 16);
     return v;
 }
 
-// The pairs turned by their angles (sign 1) or back (-1).
-template <int SP, int VEC>
-__device__ __forceinline__ void rotate(const float2 (&cs)[SP][VEC], bool interleaved, float sign, float (&a)[SP][VEC], float (&b)[SP][VEC])
+// The pairs turned by their angles, or back.
+template <bool INTERLEAVED, bool BACK, int SP, int VEC>
+__device__ __forceinline__ void rotate(const float2 (&cs)[SP][VEC], float (&a)[SP][VEC], float (&b)[SP][VEC])
 {
 #pragma unroll
     for (int i = 0; i < SP; ++i) {
-        if (interleaved && VEC > 1) {
+        if constexpr (INTERLEAVED && VEC > 1) {
 #pragma unroll
             for (int e = 0; e < VEC; e += 2) {
                 const float2 u = cs[i][e / 2], v = cs[i][VEC / 2 + e / 2];
-                const float us = sign * u.y, vs = sign * v.y;
                 const float a0 = a[i][e], a1 = a[i][e + 1], b0 = b[i][e], b1 = b[i][e + 1];
-                a[i][e] = a0 * u.x - a1 * us;
-                a[i][e + 1] = a1 * u.x + a0 * us;
-                b[i][e] = b0 * v.x - b1 * vs;
-                b[i][e + 1] = b1 * v.x + b0 * vs;
+                a[i][e] = BACK ? a0 * u.x + a1 * u.y : a0 * u.x - a1 * u.y;
+                a[i][e + 1] = BACK ? a1 * u.x - a0 * u.y : a1 * u.x + a0 * u.y;
+                b[i][e] = BACK ? b0 * v.x + b1 * v.y : b0 * v.x - b1 * v.y;
+                b[i][e + 1] = BACK ? b1 * v.x - b0 * v.y : b1 * v.x + b0 * v.y;
             }
         } else {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float c = cs[i][e].x, s = sign * cs[i][e].y, x = a[i][e], y = b[i][e];
-                a[i][e] = x * c - y * s;
-                b[i][e] = y * c + x * s;
+                const float2 u = cs[i][e];
+                const float x = a[i][e], y = b[i][e];
+                a[i][e] = BACK ? x * u.x + y * u.y : x * u.x - y * u.y;
+                b[i][e] = BACK ? y * u.x - x * u.y : y * u.x + x * u.y;
             }
         }
     }
 }
 
-// Cosines and sines of a lane's pairs at a row's position: exact products, whole turns dropped.  The waves come from L1 (12 registers
-// less than keeping them, and a third block on the SM).
+// Cosines and sines of a lane's pairs at a row's position: exact products, whole turns dropped.  The waves come from L1 (that
+// is 12 registers less than keeping them).
 template <class T, int VEC, int SP, int C>
 __device__ __forceinline__ void row_angles(const HeadArgs &p, const float *waves, int lane, const float (&pos)[3], float2 (&cs)[SP][VEC])
 {
@@ -130,8 +137,8 @@ __device__ __forceinline__ void row_angles(const HeadArgs &p, const float *waves
 }
 
 // Forward and backward: groups of lanes walk the rows, each with one unit of every row's heads.
-template <class T, int VEC, int SP, bool BWD>
-__global__ void __launch_bounds__(THREADS, SP > 1 ? 1 : BWD || VEC == 8 ? 2 : 3) qk_norm_kernel(const HeadArgs p)
+template <class T, int VEC, int SP, bool INTERLEAVED, bool BWD>
+__global__ void __launch_bounds__(THREADS, SP > 1 ? 1 : 2) qk_norm_kernel(const HeadArgs p)
 {
     using R = Raw<T, VEC>;
     extern __shared__ float shared[];
@@ -139,34 +146,37 @@ __global__ void __launch_bounds__(THREADS, SP > 1 ? 1 : BWD || VEC == 8 ? 2 : 3)
     const long long group = (long long)blockIdx.x * per_block + threadIdx.x / p.lanes, walk = (long long)gridDim.x * per_block / p.units;
     const bool walks = group < walk * p.units;  // (the last few of a grid that is no multiple of the units have none)
     const int u = (int)(group % p.units), shared_by = (int)(p.d.Hq / p.d.Hk);
-    // heads of the unit: key head j, then its query heads; or one head alone
+    // heads of the unit: key head j, then its query heads; or (single) one head alone, which takes the queries' place
     const bool key_alone = p.single && u >= p.d.Hq;
     const int j = !p.single ? u : key_alone ? u - (int)p.d.Hq : u / shared_by;
-    const int heads = p.single ? 1 : 1 + shared_by;
+    const int queries = p.single ? 1 : shared_by, q0 = p.single ? (key_alone ? j : u) : j * shared_by;
 
     bool on[SP], on_b[SP];
-    Place at[SP];
-    constexpr bool KEEP = BWD || VEC == 8;  // the weights in registers; else they come from L1 head by head, for a third block on the SM
-    R wq_raw[KEEP ? SP : 1][2], wk_raw[KEEP ? SP : 1][2];  // (single: the head's in wq_raw)
-    const bool weighted_q = p.d.wq != nullptr, weighted_k = p.d.wk != nullptr;
+    int at_a[SP], to_b[SP];  // a slot's first vector in a head, and its second one from there
     const T *wq = static_cast<const T *>(key_alone ? p.d.wk : p.d.wq), *wk = static_cast<const T *>(p.d.wk);
-    if (key_alone) wq = wq == nullptr ? nullptr : wq + j * p.d.wk_head;
-    else if (wq != nullptr) wq += (p.single ? u : (long long)j * shared_by) * p.d.wq_head;
-    if (wk != nullptr) wk += j * p.d.wk_head;
+    if (wq != nullptr) wq += (long long)q0 * (key_alone ? p.d.wk_head : p.d.wq_head);
+    if (wk != nullptr) wk += (long long)j * p.d.wk_head;
+    R wq_raw[SP][2], wk_raw[SP][2];  // the weights, as they lie in memory
 #pragma unroll
     for (int i = 0; i < SP; ++i) {
         const int slot = lane + i * p.lanes;
         on[i] = slot < p.slots;
-        at[i] = place_of<VEC>(p, on[i] ? slot : 0);
-        on_b[i] = on[i] && at[i].has_b;
-        if constexpr (KEEP) {
-            wq_raw[i][0] = wq_raw[i][1] = wk_raw[i][0] = wk_raw[i][1] = R{};
-            if (wq != nullptr && on[i]) wq_raw[i][0] = load_raw<T, VEC>(wq + at[i].a);
-            if (wq != nullptr && on_b[i]) wq_raw[i][1] = load_raw<T, VEC>(wq + at[i].b);
-            if (wk != nullptr && on[i]) wk_raw[i][0] = load_raw<T, VEC>(wk + at[i].a);
-            if (wk != nullptr && on_b[i]) wk_raw[i][1] = load_raw<T, VEC>(wk + at[i].b);
-        }
+        const Place at = place_of<VEC>(p, on[i] ? slot : 0);
+        on_b[i] = on[i] && at.has_b;
+        at_a[i] = at.a;
+        to_b[i] = at.b - at.a;
     }
+    auto weights = [&](const T *w, R(&raw)[SP][2]) {
+#pragma unroll
+        for (int i = 0; i < SP; ++i) {
+            raw[i][0] = raw[i][1] = R{};
+            if (w != nullptr && on[i]) raw[i][0] = load_raw<T, VEC>(w + at_a[i]);
+            if (w != nullptr && on_b[i]) raw[i][1] = load_raw<T, VEC>(w + at_a[i] + to_b[i]);
+        }
+    };
+    weights(wq, wq_raw);
+    weights(wk, wk_raw);
+    const bool weighted_q = wq != nullptr, weighted_k = wk != nullptr;
     const float inv_d = 1.f / (float)D, eps = (float)p.d.eps;
     float sum_q[BWD ? SP : 1][2][VEC], sum_k[BWD ? SP : 1][2][VEC];
     if constexpr (BWD) {
@@ -178,135 +188,140 @@ __global__ void __launch_bounds__(THREADS, SP > 1 ? 1 : BWD || VEC == 8 ? 2 : 3)
     // (all lanes of a warp make the same number of steps: those without a row repeat the last one and keep nothing)
     const int N = (int)p.d.N, row0 = walks ? (int)(group / p.units) : N, steps = walk > 0 ? (int)((N + walk - 1) / walk) : 0;
     auto row_of = [&](int step) { return (int)min(row0 + step * walk, (long long)N - 1); };
-    // the heads' places in a row: key head j, query heads of it (single: the one head, in the queries' place)
-    const int q0 = p.single ? (key_alone ? j : u) : j * shared_by;
+    // the unit's places in a row, of inputs and (contiguous) of outputs and their gradients
     const T *kx = static_cast<const T *>(p.d.k) + (long long)j * p.d.k_head;
     const T *qx = key_alone ? kx : static_cast<const T *>(p.d.q) + (long long)q0 * p.d.q_head;
     const int k_row = (int)p.d.k_row, q_row = key_alone ? k_row : (int)p.d.q_row, q_head = (int)p.d.q_head;
     const int k_out_row = (int)p.d.Hk * D, q_out_row = key_alone ? k_out_row : (int)p.d.Hq * D;
-    const T *gkx = static_cast<const T *>(p.gk_out) + j * D, *gqx = key_alone ? gkx : static_cast<const T *>(p.gq_out) + q0 * D;
+    const T *gk = static_cast<const T *>(p.gk_out) + j * D, *gq = key_alone ? gk : static_cast<const T *>(p.gq_out) + q0 * D;
     T *ky = static_cast<T *>(p.k_out) + j * D, *qy = key_alone ? ky : static_cast<T *>(p.q_out) + q0 * D;
     R xa[SP], xb[SP], ga[BWD ? SP : 1], gb[BWD ? SP : 1];
-    float pos[3];
-    auto fetch = [&](int step, int i) {
-        const int n = row_of(step);
-        const bool of_k = !p.single && i == 0;
-        const int at_q = p.single ? 0 : i - 1;
-        const T *x = of_k ? kx + (long long)n * k_row : qx + (long long)n * q_row + at_q * q_head;
-        const T *g = nullptr;
-        if constexpr (BWD) g = of_k ? gkx + (long long)n * k_out_row : gqx + (long long)n * q_out_row + at_q * D;
+    auto fetch = [&](const T *x, const T *g) {
 #pragma unroll
         for (int s = 0; s < SP; ++s) {
             xa[s] = xb[s] = R{};
-            if (on[s]) xa[s] = load_raw<T, VEC>(x + at[s].a);
-            if (on_b[s]) xb[s] = load_raw<T, VEC>(x + at[s].b);
+            const T *from = x + at_a[s];
+            if (on[s]) xa[s] = load_raw<T, VEC>(from);
+            if (on_b[s]) xb[s] = load_raw<T, VEC>(from + to_b[s]);
             if constexpr (BWD) {
                 ga[s] = gb[s] = R{};
-                if (on[s]) ga[s] = load_raw<T, VEC>(g + at[s].a);
-                if (on_b[s]) gb[s] = load_raw<T, VEC>(g + at[s].b);
+                const T *gf = g + at_a[s];
+                if (on[s]) ga[s] = load_raw<T, VEC>(gf);
+                if (on_b[s]) gb[s] = load_raw<T, VEC>(gf + to_b[s]);
             }
         }
-        if (i == 0) {
-#pragma unroll
-            for (int c = 0; c < 3; ++c) pos[c] = p.d.P > 0 && c < C ? p.d.pos[(long long)n * C + c] : 0.f;
+    };
+    float pos[3] = {0.f, 0.f, 0.f};
+    auto fetch_row = [&](int n) {
+        if (p.single) fetch(qx + (long long)n * q_row, gq + (long long)n * q_out_row);
+        else fetch(kx + (long long)n * k_row, gk + (long long)n * k_out_row);
+        if (p.d.P > 0) {
+            const float *from = p.d.pos + (long long)n * C;
+            pos[0] = from[0];
+            if (C > 1) pos[1] = from[1];
+            if (C > 2) pos[2] = from[2];
         }
     };
-    if (steps > 0) fetch(0, 0);
-    const float *wave0 = p.d.waves + (p.d.wave_heads == 1 ? 0 : (long long)j) * p.d.P * C;
     float2 cs[SP][VEC];
+    float a[SP][VEC], b[SP][VEC], fa[BWD ? SP : 1][VEC], fb[BWD ? SP : 1][VEC];
+    auto take = [&]() {
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+            expand<T, VEC>(xa[s], a[s]);
+            expand<T, VEC>(xb[s], b[s]);
+            if constexpr (BWD) {
+                expand<T, VEC>(ga[s], fa[s]);
+                expand<T, VEC>(gb[s], fb[s]);
+            }
+        }
+    };
+    // one head, taken: its norm, weights and rotation, or the gradients'
+    auto head = [&](const R(&w)[SP][2], bool weighted, auto &sum, T *to, bool live) {
+        float square = 0.f;
+#pragma unroll
+        for (int s = 0; s < SP; ++s)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) square += a[s][e] * a[s][e] + b[s][e] * b[s][e];
+        if constexpr (BWD) rotate<INTERLEAVED, true>(cs, fa, fb);
+        const float r = rsqrtf(lanes_sum(square, p.lanes) * inv_d + eps);
+#pragma unroll
+        for (int s = 0; s < SP; ++s)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) { a[s][e] *= r; b[s][e] *= r; }  // x r from here on
+        if (weighted) {
+#pragma unroll
+            for (int s = 0; s < SP; ++s) {
+                float wa[VEC], wb[VEC];
+                expand<T, VEC>(w[s][0], wa);
+                expand<T, VEC>(w[s][1], wb);
+                if constexpr (!BWD) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) { a[s][e] *= wa[e]; b[s][e] *= wb[e]; }
+                } else {
+                    if (live) {  // (a value that is no number belongs to its own row's sums alone)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) { sum[s][0][e] += fa[s][e] * a[s][e]; sum[s][1][e] += fb[s][e] * b[s][e]; }
+                    }
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) { fa[s][e] *= wa[e]; fb[s][e] *= wb[e]; }
+                }
+            }
+        }
+        if constexpr (!BWD) {
+            rotate<INTERLEAVED, false>(cs, a, b);
+        } else {
+            float dot = 0.f;
+#pragma unroll
+            for (int s = 0; s < SP; ++s)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) dot += a[s][e] * fa[s][e] + b[s][e] * fb[s][e];
+            const float m = lanes_sum(dot, p.lanes) * inv_d;
+#pragma unroll
+            for (int s = 0; s < SP; ++s)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    a[s][e] = r * (fa[s][e] - a[s][e] * m);
+                    b[s][e] = r * (fb[s][e] - b[s][e] * m);
+                }
+        }
+        if (live) {
+#pragma unroll
+            for (int s = 0; s < SP; ++s) {
+                T *at = to + at_a[s];
+                if (on[s]) store_values<T, VEC>(at, a[s]);
+                if (on_b[s]) store_values<T, VEC>(at + to_b[s], b[s]);
+            }
+        }
+    };
+    const float *wave0 = p.d.waves + (p.d.wave_heads == 1 ? 0 : (long long)j) * p.d.P * C;
+    if (steps > 0) fetch_row(row_of(0));
     for (int step = 0; step < steps; ++step) {
         const bool live = row0 + step * walk < N;
         const int n = row_of(step);
         if (C == 3) row_angles<T, VEC, SP, 3>(p, wave0, lane, pos, cs);
         else if (C == 2) row_angles<T, VEC, SP, 2>(p, wave0, lane, pos, cs);
         else row_angles<T, VEC, SP, 1>(p, wave0, lane, pos, cs);
-        for (int i = 0; i < heads; ++i) {
-            float a[SP][VEC], b[SP][VEC], fa[BWD ? SP : 1][VEC], fb[BWD ? SP : 1][VEC];
-            float square = 0.f;
-#pragma unroll
-            for (int s = 0; s < SP; ++s) {
-                expand<T, VEC>(xa[s], a[s]);
-                expand<T, VEC>(xb[s], b[s]);
-                if constexpr (BWD) {
-                    expand<T, VEC>(ga[s], fa[s]);
-                    expand<T, VEC>(gb[s], fb[s]);
-                }
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) square += a[s][e] * a[s][e] + b[s][e] * b[s][e];
+        const T *x = qx + (long long)n * q_row;
+        const long long out = (long long)n * q_out_row;
+        const T *g = gq + out;
+        T *y = qy + out;
+        // a head's values are taken, the next one's fetched, then it is computed
+        if (!p.single) {
+            take();
+            fetch(x, g);
+            head(wk_raw, weighted_k, sum_k, ky + (long long)n * k_out_row, live);
+        }
+        for (int i = 0; i < queries; ++i) {
+            take();
+            if (i + 1 < queries) {
+                x += q_head;
+                g += D;
+                fetch(x, g);
+            } else if (step + 1 < steps) {
+                fetch_row(row_of(step + 1));
             }
-            // the next head's values, then the next row's
-            const bool last = i + 1 == heads;
-            if (!last || step + 1 < steps) fetch(last ? step + 1 : step, last ? 0 : i + 1);
-            const bool of_k = !p.single && i == 0, weighted = key_alone || of_k ? weighted_k : weighted_q;
-            R wa_raw[SP], wb_raw[SP];
-#pragma unroll
-            for (int s = 0; s < SP; ++s) {
-                if constexpr (KEEP) {
-                    wa_raw[s] = choose(of_k, wk_raw[s][0], wq_raw[s][0]);
-                    wb_raw[s] = choose(of_k, wk_raw[s][1], wq_raw[s][1]);
-                } else {
-                    wa_raw[s] = wb_raw[s] = R{};
-                    const T *w = of_k ? wk : wq;
-                    if (weighted && on[s]) wa_raw[s] = load_raw<T, VEC>(w + at[s].a);
-                    if (weighted && on_b[s]) wb_raw[s] = load_raw<T, VEC>(w + at[s].b);
-                }
-            }
-            const float r = rsqrtf(lanes_sum(square, p.lanes) * inv_d + eps);
-            T *to = of_k ? ky + (long long)n * k_out_row : qy + (long long)n * q_out_row + (p.single ? 0 : i - 1) * D;
-            if constexpr (!BWD) {
-#pragma unroll
-                for (int s = 0; s < SP; ++s) {
-                    float wa[VEC], wb[VEC];
-                    expand<T, VEC>(wa_raw[s], wa);
-                    expand<T, VEC>(wb_raw[s], wb);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        a[s][e] *= r;
-                        b[s][e] *= r;
-                        if (weighted) { a[s][e] *= wa[e]; b[s][e] *= wb[e]; }
-                    }
-                }
-                rotate(cs, p.d.interleaved, 1.f, a, b);
-            } else {
-                rotate(cs, p.d.interleaved, -1.f, fa, fb);
-                float dot = 0.f;
-#pragma unroll
-                for (int s = 0; s < SP; ++s) {
-                    float wa[VEC], wb[VEC];
-                    expand<T, VEC>(wa_raw[s], wa);
-                    expand<T, VEC>(wb_raw[s], wb);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        a[s][e] *= r;  // x r from here on
-                        b[s][e] *= r;
-                        if (weighted) {
-                            if (live) {  // (a value that is no number belongs to its own row's sums alone)
-                                const float ta = fa[s][e] * a[s][e], tb = fb[s][e] * b[s][e];
-                                if (of_k) { sum_k[s][0][e] += ta; sum_k[s][1][e] += tb; }
-                                else { sum_q[s][0][e] += ta; sum_q[s][1][e] += tb; }
-                            }
-                            fa[s][e] *= wa[e];
-                            fb[s][e] *= wb[e];
-                        }
-                        dot += a[s][e] * fa[s][e] + b[s][e] * fb[s][e];
-                    }
-                }
-                const float m = lanes_sum(dot, p.lanes) * inv_d;
-#pragma unroll
-                for (int s = 0; s < SP; ++s)
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        a[s][e] = r * (fa[s][e] - a[s][e] * m);
-                        b[s][e] = r * (fb[s][e] - b[s][e] * m);
-                    }
-            }
-            if (live) {
-#pragma unroll
-                for (int s = 0; s < SP; ++s) {
-                    if (on[s]) store_values<T, VEC>(to + at[s].a, a[s]);
-                    if (on_b[s]) store_values<T, VEC>(to + at[s].b, b[s]);
-                }
-            }
+            head(wq_raw, weighted_q, sum_q, y, live);
+            y += D;
         }
     }
     if constexpr (BWD) {
@@ -321,8 +336,8 @@ __global__ void __launch_bounds__(THREADS, SP > 1 ? 1 : BWD || VEC == 8 ? 2 : 3)
                 for (int s = 0; s < SP; ++s) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
-                        if (on[s]) mine[at[s].a + e] = which ? sum_k[s][0][e] : sum_q[s][0][e];
-                        if (on_b[s]) mine[at[s].b + e] = which ? sum_k[s][1][e] : sum_q[s][1][e];
+                        if (on[s]) mine[at_a[s] + e] = which ? sum_k[s][0][e] : sum_q[s][0][e];
+                        if (on_b[s]) mine[at_a[s] + to_b[s] + e] = which ? sum_k[s][1][e] : sum_q[s][1][e];
                     }
                 }
                 __syncthreads();
@@ -421,7 +436,7 @@ int units_of(const cf_qk_norm &d, int &single)
     return (int)(single ? d.Hq + d.Hk : d.Hk);
 }
 
-template <class T, int VEC, int SP, bool BWD>
+template <class T, int VEC, int SP, bool INTERLEAVED, bool BWD>
 int launch_sp(const HeadArgs &a, void *gwq, void *gwk, cudaStream_t s)
 {
     static thread_local int resident[64] = {};
@@ -431,20 +446,20 @@ int launch_sp(const HeadArgs &a, void *gwq, void *gwk, cudaStream_t s)
     cudaGetDevice(&dev);
     int &at_once = resident[dev & 63];
     if (at_once == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, qk_norm_kernel<T, VEC, SP, BWD>, THREADS, 16384) != cudaSuccess || at_once < 1) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, qk_norm_kernel<T, VEC, SP, INTERLEAVED, BWD>, THREADS, 16384) != cudaSuccess || at_once < 1) {
             cudaGetLastError();
             at_once = 1;
         }
         if (at_once > MAX_BLOCKS_PER_SM) at_once = MAX_BLOCKS_PER_SM;
     }
     const long long blocks = blocks_of(a.d.N * a.units, a.units, per_block, at_once);
-    qk_norm_kernel<T, VEC, SP, BWD><<<(unsigned)blocks, THREADS, smem, s>>>(a);
+    qk_norm_kernel<T, VEC, SP, INTERLEAVED, BWD><<<(unsigned)blocks, THREADS, smem, s>>>(a);
     if (BWD && a.partial != nullptr)
         qk_weight_sum_kernel<T><<<(a.columns + 31) / 32, 1024, 0, s>>>(a.partial, (int)blocks, a.columns, a.columns_q, static_cast<T *>(gwq), static_cast<T *>(gwk));
     return launch_status("qk_norm_kernel");
 }
 
-template <class T, int VEC, bool BWD>
+template <class T, int VEC, bool INTERLEAVED, bool BWD>
 int launch_vec(HeadArgs a, void *gwq, void *gwk, cudaStream_t s)
 {
     a.rotated = (int)(a.d.P / VEC);
@@ -452,20 +467,21 @@ int launch_vec(HeadArgs a, void *gwq, void *gwk, cudaStream_t s)
     a.lanes = 1;
     while (a.lanes < 32 && a.lanes < a.slots) a.lanes *= 2;
     const int sp = (a.slots + a.lanes - 1) / a.lanes;
-    if (sp <= 1) return launch_sp<T, VEC, 1, BWD>(a, gwq, gwk, s);
-    if constexpr (VEC <= 4) if (sp <= 2) return launch_sp<T, VEC, 2, BWD>(a, gwq, gwk, s);  // (heads of up to 512: 64 slots of 8 values, 256 of 2)
-    if constexpr (VEC == 1) return launch_sp<T, VEC, 8, BWD>(a, gwq, gwk, s);
+    if (sp <= 1) return launch_sp<T, VEC, 1, INTERLEAVED, BWD>(a, gwq, gwk, s);
+    if constexpr (VEC <= 4) if (sp <= 2) return launch_sp<T, VEC, 2, INTERLEAVED, BWD>(a, gwq, gwk, s);  // (heads of up to 512: 64 slots of 8 values, 256 of 2)
+    if constexpr (VEC == 1) return launch_sp<T, VEC, 8, INTERLEAVED, BWD>(a, gwq, gwk, s);
     return fail(CF_ERR_RANGE, "cf_qk_norm: heads of %lld", (long long)a.d.D);
 }
 
 template <class T, bool BWD>
 int launch(const HeadArgs &a, void *gwq, void *gwk, cudaStream_t s)
 {
+    // (single values: pairs are taken one by one either way)
     if constexpr (sizeof(T) == 2 && !BWD) {
-        if (fits(a, 8, BWD)) return launch_vec<T, 8, BWD>(a, gwq, gwk, s);
+        if (fits(a, 8, BWD)) return a.d.interleaved ? launch_vec<T, 8, true, BWD>(a, gwq, gwk, s) : launch_vec<T, 8, false, BWD>(a, gwq, gwk, s);
     }
-    if (fits(a, 4, BWD)) return launch_vec<T, 4, BWD>(a, gwq, gwk, s);
-    return launch_vec<T, 1, BWD>(a, gwq, gwk, s);
+    if (fits(a, 4, BWD)) return a.d.interleaved ? launch_vec<T, 4, true, BWD>(a, gwq, gwk, s) : launch_vec<T, 4, false, BWD>(a, gwq, gwk, s);
+    return launch_vec<T, 1, false, BWD>(a, gwq, gwk, s);
 }
 
 template <bool BWD>

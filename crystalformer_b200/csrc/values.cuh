@@ -92,13 +92,6 @@ template <> struct RawBytes<4> { using type = uint32_t; };
 template <> struct RawBytes<2> { using type = uint16_t; };
 template <class T, int VEC> using Raw = typename RawBytes<VEC * sizeof(T)>::type;
 template <class T, int VEC> __device__ __forceinline__ Raw<T, VEC> load_raw(const T *p) { return *reinterpret_cast<const Raw<T, VEC> *>(p); }
-__device__ __forceinline__ uint16_t choose(bool first, uint16_t a, uint16_t b) { return first ? a : b; }
-__device__ __forceinline__ uint32_t choose(bool first, uint32_t a, uint32_t b) { return first ? a : b; }
-__device__ __forceinline__ uint2 choose(bool first, const uint2 &a, const uint2 &b) { return make_uint2(first ? a.x : b.x, first ? a.y : b.y); }
-__device__ __forceinline__ uint4 choose(bool first, const uint4 &a, const uint4 &b)
-{
-    return make_uint4(first ? a.x : b.x, first ? a.y : b.y, first ? a.z : b.z, first ? a.w : b.w);  // (in registers: an address is not taken)
-}
 template <class T> __device__ __forceinline__ float value_of(uint32_t w) { return __uint_as_float(w); }  // of a word with one value
 template <> __device__ __forceinline__ float value_of<__nv_bfloat16>(uint32_t w) { return __uint_as_float(w << 16); }
 template <> __device__ __forceinline__ float value_of<__half>(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)w)); }
