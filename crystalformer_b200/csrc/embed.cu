@@ -210,6 +210,31 @@ __global__ void __launch_bounds__(SORT_THREADS) digit_count_kernel(const int64_t
     if (threadIdx.x < 256) counts[(size_t)blockIdx.x * 256 + threadIdx.x] = mine[threadIdx.x];
 }
 
+// Where there are many blocks of rows: their counts of each digit become those of the blocks before, and the sums over all follow them
+// as one more row (each block of the pass reading all blocks' counts itself is quicker up to SCAN_BLOCKS and quadratic).  32 digits per
+// block, a share of the rows' blocks per warp.
+constexpr unsigned SCAN_BLOCKS = 128;
+__global__ void __launch_bounds__(1024) digit_scan_kernel(uint32_t *counts, unsigned blocks)
+{
+    __shared__ uint32_t part[32][33];
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
+    const unsigned lo = (unsigned)((unsigned long long)blocks * warp / 32), hi = (unsigned)((unsigned long long)blocks * (warp + 1) / 32);
+    uint32_t sum = 0u;
+#pragma unroll 8
+    for (unsigned b = lo; b < hi; ++b) sum += counts[(size_t)b * 256 + d];
+    part[warp][lane] = sum;
+    __syncthreads();
+    uint32_t before = 0u;
+    for (unsigned w = 0; w < warp; ++w) before += part[w][lane];
+#pragma unroll 8
+    for (unsigned b = lo; b < hi; ++b) {
+        const uint32_t c = counts[(size_t)b * 256 + d];
+        counts[(size_t)b * 256 + d] = before;
+        before += c;
+    }
+    if (warp == 31) counts[(size_t)blocks * 256 + d] = before;
+}
+
 // One pass: rows to their places by eight bits of their keys, equal digits in their present order; `next`: the counts of the next
 // pass' blocks.
 __global__ void __launch_bounds__(SORT_THREADS) digit_place_kernel(const int64_t *ids, const uint32_t *keys, const uint32_t *rows, long long N,
@@ -228,12 +253,19 @@ __global__ void __launch_bounds__(SORT_THREADS) digit_place_kernel(const int64_t
     }
     // counts of digit d, of the blocks before this one and of all: half of the blocks each
     uint32_t total = 0u, earlier = 0u;
-    const unsigned mid = (gridDim.x + 1) / 2, lo = part ? mid : 0u, hi = part ? gridDim.x : mid;
+    if (gridDim.x > SCAN_BLOCKS) {  // (digit_scan_kernel has been there)
+        if (!part) {
+            total = counts[(size_t)gridDim.x * 256 + d];
+            earlier = counts[(size_t)blockIdx.x * 256 + d];
+        }
+    } else {
+        const unsigned mid = (gridDim.x + 1) / 2, lo = part ? mid : 0u, hi = part ? gridDim.x : mid;
 #pragma unroll 16
-    for (unsigned b = lo; b < hi; ++b) {
-        const uint32_t c = counts[(size_t)b * 256 + d];
-        total += c;
-        earlier += b < blockIdx.x ? c : 0u;
+        for (unsigned b = lo; b < hi; ++b) {
+            const uint32_t c = counts[(size_t)b * 256 + d];
+            total += c;
+            earlier += b < blockIdx.x ? c : 0u;
+        }
     }
     for (int w = part; w < SORT_WARPS; w += 2) seen[w][d] = 0u;
     __syncthreads();
@@ -459,7 +491,7 @@ struct EmbedWork {
     EmbedWork(void *base, long long N, long long D)
     {
         Carver c{static_cast<char *>(base)};
-        counts_of = (size_t)((N + SORT_TILE - 1) / SORT_TILE) * 256;
+        counts_of = (size_t)((N + SORT_TILE - 1) / SORT_TILE + 1) * 256;  // (a row for the sums)
         counts = c.take<uint32_t>(4 * counts_of);
         runs = c.take<uint32_t>((size_t)((N + CHUNK - 1) / CHUNK) + 1);
         for (int i = 0; i < 2; ++i) { keys[i] = c.take<uint32_t>(N); rows[i] = c.take<uint32_t>(N); }
@@ -527,6 +559,7 @@ int cf_embed_bwd(const void *gout, int64_t ld, int type, const int64_t *ids, int
     for (int shift = 0, pass = 0; shift < 32 && (V >> shift) != 0; shift += 8, ++pass) {
         const bool more = shift + 8 < 32 && (V >> (shift + 8)) != 0;
         uint32_t *counts = w.counts + pass * w.counts_of;
+        if (blocks > SCAN_BLOCKS) digit_scan_kernel<<<8, 1024, 0, s>>>(counts, blocks);
         digit_place_kernel<<<blocks, SORT_THREADS, 0, s>>>(ids, keys, rows, N, V, shift, counts, more ? counts + w.counts_of : nullptr, w.keys[pass & 1],
                                                            w.rows[pass & 1]);
         keys = w.keys[pass & 1];

@@ -70,6 +70,14 @@ def test_lookup_and_gradient(N, V, D, dtype):
             check(table.detach(), ids, gout, out.detach(), grad, 0.25)
 
 
+@pytest.mark.parametrize("N,V,D", [(262145, 70001, 8), (600001, 98, 16), (1000003, 300, 3)])
+def test_many_rows(N, V, D):
+    """More blocks of rows than the sort's passes read the counts of themselves."""
+    from crystalformer_b200 import ops
+    table, ids, gout = make(N, V, D, torch.float32, 4, padding=True)
+    check(table, ids, gout, ops.embed_fwd(ids, table, 0.5), ops.embed_bwd(ids, gout, V, 0.5), 0.5)
+
+
 def test_layout_of_the_gradient():
     """The gradient reaches the weight of a Linear contiguous."""
     from crystalformer_b200.embedding import embed_species
