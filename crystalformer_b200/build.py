@@ -74,7 +74,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return LIB_PATH
     nvcc = os.environ.get("NVCC", "nvcc")
-    cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + SOURCES + ["-o", LIB_PATH]
+    cmd = [nvcc, "--threads", "0"] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + SOURCES + ["-o", LIB_PATH]
     env = dict(os.environ)
     # the host compiler must be the system gcc
     env["PATH"] = "/usr/bin:" + env.get("PATH", "")

@@ -319,8 +319,10 @@ class Latticeformer(nn.Module):
         one-call path only): a CUDA event after which the tensors of ``data`` are valid.  The batch preparation, which
         depends on the inputs alone, is then not ordered behind the work already queued on the current stream and
         overlaps the previous batch's forward; the tensors must stay unchanged until this forward has run."""
-        species = species_of(data)
-        onehot = species is getattr(data, "x", None)
+        species = getattr(data, "x", None)
+        onehot = species is not None
+        if not onehot:
+            species = data.z
         if onehot and geometry is None and not self.training and not torch.is_grad_enabled() and data.pos.is_cuda \
                 and self._native_ok():
             return self._forward_native(data, counts, gather, inputs_ready=inputs_ready)

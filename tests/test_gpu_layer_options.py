@@ -195,6 +195,47 @@ def test_a_captured_step_of_the_operators_together():
         assert (a.double() - b.double()).norm() <= 24 * 2.0 ** -9 * 2 * b.double().norm()
 
 
+FRESH = """
+import torch
+from crystalformer_b200 import ops
+from crystalformer_b200.embedding import embed_species
+from crystalformer_b200.feedforward import gated_feed_forward
+from crystalformer_b200.qk_norm import normalize_rotate
+torch.manual_seed(0)
+r = lambda *s: torch.randn(s, device="cuda")
+table, ids, pos, waves = r(9, 128), torch.randint(0, 9, (300,), device="cuda"), torch.rand((300, 3), device="cuda"), torch.ones((1, 8, 3), device="cuda")
+w = [r(512, 128) * 0.1, r(512, 128) * 0.1, r(128, 512) * 0.1]
+leaves = [t.requires_grad_() for t in (table, *w)]
+gout = r(300, 128)
+def step():
+    x = embed_species(ids, table, 0.5)
+    q, k = normalize_rotate(x.view(300, 8, 16), x.view(300, 8, 16), None, None, pos, waves)
+    y = gated_feed_forward((q + k).reshape(300, 128), *w)
+    return (y, *torch.autograd.grad(y, leaves, gout))
+graph = torch.cuda.CUDAGraph()
+torch.zeros(1, device="cuda").add_(1)  # (a context; none of the library's kernels has run)
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    captured = step()
+graph.replay()
+torch.cuda.synchronize()
+captured = [t.clone() for t in captured]
+eager = step()
+assert all(torch.equal(a, b) for a, b in zip(captured, eager))
+ops.set_chained_launches(False)
+assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+print("the same")
+"""
+
+
+def test_a_process_that_starts_with_a_capture():
+    """The first calls of a process may be captured ones; results do not depend on how the kernels of a call are chained."""
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, "-c", FRESH], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
+
+
 def test_refusals():
     from crystalformer_b200.model import Latticeformer, default_params
     with pytest.raises(NotImplementedError):
