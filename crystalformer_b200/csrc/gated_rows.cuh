@@ -21,15 +21,6 @@ namespace rows {
 
 constexpr int THREADS = 256;
 
-template <class T, int VEC>
-__device__ __forceinline__ void load_row(const T *p, int room, float (&v)[VEC])
-{
-    if constexpr (VEC > 1) {
-        load_values<T, VEC>(p, v);
-    } else {
-        v[0] = room > 0 ? to_float(*p) : 0.f;
-    }
-}
 template <int VEC>
 __device__ __forceinline__ void load_hidden(const float *p, float (&v)[VEC])
 {
@@ -196,7 +187,8 @@ __device__ __forceinline__ void mma_32(float (&c)[4], const uint4 &lo, const uin
 }
 
 // MATS matrices of (M, K) weights by up to eight rows x (ld) of K values: sums[mat][unit of 16][row of 8] of the block's 16 units in
-// `part`, (warps, MATS, 16, 8).  MMA_AHEAD: steps of 32 on their way.  `wait`: x comes from the kernel before (the weights are the caller's, and may be fetched earlier).
+// `part`, (warps, MATS, 16, 8).  MMA_AHEAD: steps of 32 on their way.  WAIT: x comes from the kernel before (the weights are the
+// caller's, and are fetched earlier).
 template <class T, int MATS, int MMA_AHEAD, bool WAIT>
 __device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int K, const T *x, long long ld, int rows, int unit0, int warps, float *part)
 {

@@ -8,11 +8,6 @@
 
 namespace cf {
 
-template <class T> struct TypeCode;
-template <> struct TypeCode<float> { static constexpr int value = CF_FLOAT32; };
-template <> struct TypeCode<__nv_bfloat16> { static constexpr int value = CF_BFLOAT16; };
-template <> struct TypeCode<__half> { static constexpr int value = CF_FLOAT16; };
-
 inline bool known_type(int type) { return type == CF_FLOAT32 || type == CF_BFLOAT16 || type == CF_FLOAT16; }
 inline int type_size(int type) { return type == CF_FLOAT32 ? 4 : 2; }
 
