@@ -282,7 +282,11 @@ struct Linear {
 // How the products of one launch are cut: width of the tiles, one block or a pair of them to a tile, and into how many shares each
 // contraction.  Shares are as long as `length` blocks at most, so that the tiles of all products take about as long; the cheapest
 // length by the rounds of the launch (blocks of the contraction, and what a tile costs beside them) and by the shares' way through
-// memory.  Unit: 256 clocks, the products of 128 x 128 x 64 values of 16 bits.
+// memory.  Unit: 256 clocks, the products of 128 x 128 x 64 values of 16 bits.  Measured with each width forced (y; the three gradients):
+//   1,984 rows, 128 x 512, float32                pair 256: 25; 31 us   pair 128: 17; 22   single 64: 11; 21
+//   133,120 rows, 128 x 512, float32                       163; 669              108; 450            157; 756
+//   8,192 rows, 1024 x 2816, bfloat16                       50; 216               84; 355            133; 708
+// (single blocks of 128 x 128 were within 5 % of one of them everywhere).
 struct Size {
     long long M;
     int N, blocks;
@@ -298,7 +302,7 @@ Cut find_cut(const Size *sizes, int count)
 {
     // a block of the contraction of a 16-bit type: its products, or what L2 delivers; of float32: six products
     struct Kind { int tn; bool pair; double one, six; };
-    constexpr Kind kinds[] = {{256, true, 3.4, 20.0}, {128, true, 3.2, 11.0}, {128, false, 3.2, 13.5}, {64, false, 2.2, 7.5}};
+    constexpr Kind kinds[] = {{256, true, 3.4, 20.0}, {128, true, 3.2, 11.0}, {64, false, 2.2, 7.5}};
     constexpr bool wide = pieces_of<T> > 1;
     const double sms = sm_count();
     int most = 1;
@@ -396,8 +400,8 @@ int run_linear(const Linear *products, int count, const Cut &cut, float *partial
             tickets += (size_t)q.m_tiles * q.n_tiles * (cut.pair ? 2 : 1) * EPILOGUE_WARPS;
         }
     }
-    return cut.tn == 256 ? launch_tiles<T, LINEAR, 256, true>(p, true, s) : cut.pair ? launch_tiles<T, LINEAR, 128, true>(p, true, s) :
-           cut.tn == 128 ? launch_tiles<T, LINEAR, 128, false>(p, true, s) : launch_tiles<T, LINEAR, 64, false>(p, true, s);
+    return cut.tn == 256 ? launch_tiles<T, LINEAR, 256, true>(p, true, s) : cut.tn == 128 ? launch_tiles<T, LINEAR, 128, true>(p, true, s) :
+                           launch_tiles<T, LINEAR, 64, false>(p, true, s);
 }
 
 // ---- plans: where the operands of a call lie ------------------------------------------------------------------------------------------------
@@ -482,7 +486,9 @@ int run_glu(const Plan<T> &plan, bool backward, bool sums, cudaStream_t s)
     p.clear = plan.tickets;
     p.clear_words = (int)plan.ticket_words;
     // Tiles of pairs (256 x 128; backward in three pieces, whose sums must fit registers, 256 x 64) or of single blocks (128 x 64): the
-    // cheaper by rounds times products, single blocks' bound by L2 (16 bits).
+    // cheaper by rounds times products, single blocks' bound by L2 (16 bits).  Measured (forward; backward), pairs against single blocks:
+    // 1,984 rows, 128 x 512, float32 14; 17 us against 9; 17, 133,120 rows 183; 439 against 248; 513, 4,999 rows, 201 x 517, float16
+    // 14; 23 against 13; 21, 8,192 rows, 1024 x 2816, bfloat16 91; 173 against 156; 302.
     const int pair_tn = wide && backward ? 64 : 128;
     const double sms = sm_count();
     auto rounds = [&](int tm, int tn, double at_once) { return std::ceil((double)((d.N + tm - 1) / tm) * ((d.F + tn - 1) / tn) / at_once); };
