@@ -5,9 +5,10 @@
 // all rows; lanes walk the contraction, four weights of each unit at a time, with the rows' values from L1.
 //
 // 16-bit types: multiplying and adding in float32 would take longer than the weights need to come (31 us for four rows of 2048 x 5632,
-// whose 69 MB come in 10.6), so products are taken by mma.sync m16n8k16: 16 units by up to eight rows.  The sum does not mind which
+// whose 69 MB come in 10.6; 22 by what follows), so products are taken by mma.sync m16n8k16: 16 units by up to eight rows.  The sum does not mind which
 // k an operand calls its own: lane t of a group of four takes eight neighbours, k = 8 t .. 8 t + 7 of each 32, of its two units and of
-// its row, in one 16-byte load each, and both operands of two products are there.  A block's warps share the contraction.
+// its row, in one 16-byte load each, and both operands of two products are there.  A block's warps share the contraction.  The hidden
+// units go from one kernel to the other as two values of the type, h and what its rounding left, so that only the result is rounded (1 us).
 #pragma once
 #include "common.cuh"
 #include "tile_gemm.cuh"
@@ -188,9 +189,10 @@ __device__ __forceinline__ void mma_32(float (&c)[4], const uint4 &lo, const uin
 
 // MATS matrices of (M, K) weights by up to eight rows x (ld) of K values: sums[mat][unit of 16][row of 8] of the block's 16 units in
 // `part`, (warps, MATS, 16, 8).  MMA_AHEAD: steps of 32 on their way.  WAIT: x comes from the kernel before (the weights are the
-// caller's, and are fetched earlier).
-template <class T, int MATS, int MMA_AHEAD, bool WAIT>
-__device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int K, const T *x, long long ld, int rows, int unit0, int warps, float *part)
+// caller's, and are fetched earlier).  PIECES: x is the sum of so many matrices, `apart` values apart.
+template <class T, int MATS, int MMA_AHEAD, int PIECES, bool WAIT>
+__device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int K, const T *x, long long ld, long long apart, int rows, int unit0, int warps,
+                                           float *part)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const long long lo = (long long)min(unit0 + g, M - 1) * K + 8 * t, hi = (long long)min(unit0 + g + 8, M - 1) * K + 8 * t;
@@ -216,19 +218,23 @@ __device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int
 #pragma unroll
         for (int i = 0; i < 4; ++i) c[m][i] = 0.f;
     for (int k = k0; k < K; k += MMA_AHEAD * step) {
-        uint4 b[MMA_AHEAD];
+        uint4 b[MMA_AHEAD][PIECES];
 #pragma unroll
-        for (int i = 0; i < MMA_AHEAD; ++i) {
-            const int at = k + i * step;
-            b[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (at + 8 * t < K && g < rows) b[i] = *reinterpret_cast<const uint4 *>(xr + at);
-        }
+        for (int i = 0; i < MMA_AHEAD; ++i)
+#pragma unroll
+            for (int q = 0; q < PIECES; ++q) {
+                const int at = k + i * step;
+                b[i][q] = make_uint4(0u, 0u, 0u, 0u);
+                if (at + 8 * t < K && g < rows) b[i][q] = *reinterpret_cast<const uint4 *>(xr + q * apart + at);
+            }
 #pragma unroll
         for (int i = 0; i < MMA_AHEAD; ++i) {
             const int at = k + i * step;
             if (at >= K) break;
 #pragma unroll
-            for (int m = 0; m < MATS; ++m) mma_32<T>(c[m], a[i][m][0], a[i][m][1], b[i]);
+            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                for (int q = PIECES - 1; q >= 0; --q) mma_32<T>(c[m], a[i][m][0], a[i][m][1], b[i][q]);
             fetch(i, at + MMA_AHEAD * step);
         }
     }
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(256, 3) hidden_mma_kernel(const __grid_constan
     grid_launch_dependents();
     const int unit0 = blockIdx.x * 16, F = (int)d.F, N = (int)d.N;
     const T *const w[2] = {static_cast<const T *>(d.w_gate), static_cast<const T *>(d.w_up)};
-    weigh_rows<T, 2, 3, false>(w, F, (int)d.D, static_cast<const T *>(d.x), d.ldx, N, unit0, 8, part);
+    weigh_rows<T, 2, 3, 1, false>(w, F, (int)d.D, static_cast<const T *>(d.x), d.ldx, 0, N, unit0, 8, part);
     const int f = unit0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
     if (r >= N || f >= F) return;
     float a = 0.f, b = 0.f;
@@ -259,7 +265,12 @@ __global__ void __launch_bounds__(256, 3) hidden_mma_kernel(const __grid_constan
     }
     if (d.b_gate) a += to_float(static_cast<const T *>(d.b_gate)[f]);
     if (d.b_up) b += to_float(static_cast<const T *>(d.b_up)[f]);
-    h[(long long)r * F + f] = from_float<T>(activation(d.activation, a) * b);
+    const float v = activation(d.activation, a) * b;
+    const T whole = from_float<T>(v);
+    const float left = v - to_float(whole);
+    T *to = h + (long long)r * F + f;
+    to[0] = whole;
+    to[(long long)N * F] = from_float<T>(left == left ? left : 0.f);  // (an infinity leaves none)
 }
 
 template <class T>
@@ -269,7 +280,7 @@ __global__ void __launch_bounds__(512) output_mma_kernel(const __grid_constant__
     grid_launch_dependents();
     const int unit0 = blockIdx.x * 16, D = (int)d.D, N = (int)d.N;
     const T *const w[1] = {static_cast<const T *>(d.w_down)};
-    weigh_rows<T, 1, 6, true>(w, D, (int)d.F, h, d.F, N, unit0, 16, part);
+    weigh_rows<T, 1, 6, 2, true>(w, D, (int)d.F, h, d.F, (long long)N * d.F, N, unit0, 16, part);
     const int c = unit0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
     if (r >= N || c >= D) return;
     float a = 0.f;
@@ -300,7 +311,7 @@ int launch(const cf_gated_ffn &d, void *y, float *h, cudaStream_t s)
 
 }  // namespace rows
 
-// y of up to GATED_ROWS rows; h: N F floats (or, by mma.sync, values of the type: rounded once, as by the tiles).
+// y of up to GATED_ROWS rows; h: N F floats (or, by mma.sync, 2 N F values of the type).
 template <class T>
 int gated_rows(const cf_gated_ffn &d, void *y, float *h, cudaStream_t s)
 {
