@@ -180,3 +180,55 @@ def test_refusals():
     (grad,) = torch.autograd.grad(out, table, gout.requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError):  # (once differentiable)
         grad.sum().backward()
+
+
+def test_offsets_beyond_32_bits():
+    from crystalformer_b200 import ops
+    # rows of a table and of a gradient 2^28 values apart
+    far = torch.zeros(8 * 2 ** 28 + 64, dtype=torch.bfloat16, device="cuda")
+    view = far.as_strided((9, 64), (2 ** 28, 1))
+    view.copy_(torch.randn((9, 64), device="cuda"))
+    ids = torch.tensor([8, 0, 3, 8, -1, 7], device="cuda")
+    assert torch.equal(ops.embed_fwd(ids, view), ops.embed_fwd(ids, view.contiguous()))
+    nine = torch.arange(9, device="cuda") % 4
+    assert torch.equal(ops.embed_bwd(nine, view, 5), ops.embed_bwd(nine, view.contiguous(), 5))
+    del far, view
+    # an output of more than 2^31 values, and its gradient's rows
+    N, D = 2 ** 24 + 77, 128
+    table = torch.randn((98, D), device="cuda").bfloat16()
+    ids = torch.randint(0, 98, (N,), device="cuda")
+    out = ops.embed_fwd(ids, table)
+    for part in (slice(0, 1000), slice(2 ** 24 - 500, 2 ** 24 + 77)):
+        assert torch.equal(out[part], table[ids[part]])
+    out[:-50] = 0
+    grad = ops.embed_bwd(ids, out, 98)  # (the last fifty rows alone are not zero)
+    expected = torch.zeros((98, D), device="cuda").index_add_(0, ids[-50:], out[-50:].float())
+    assert (grad.float() - expected).abs().max() <= (2.0 ** -9 + 50 * 2.0 ** -24) * 2 * expected.abs().max()
+
+
+def test_from_several_threads():
+    """Calls of several host threads at once, each on its own stream."""
+    import threading
+
+    from crystalformer_b200 import ops
+    from crystalformer_b200.feedforward import gated_feed_forward
+    data = [make(3000 + 100 * i, 98, 64, torch.float32, i) for i in range(4)]
+    w = [torch.randn(s, device="cuda") * 0.1 for s in ((96, 64), (96, 64), (64, 96))]
+    alone = [(ops.embed_bwd(ids, gout, 98), gated_feed_forward(gout, *w)) for _, ids, gout in data]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        _, ids, gout = data[i]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                a, b = ops.embed_bwd(ids, gout, 98), gated_feed_forward(gout, *w)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(a, alone[i][0]) and torch.equal(b, alone[i][1])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

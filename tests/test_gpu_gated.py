@@ -292,3 +292,17 @@ def test_refusals():
     (gx,) = torch.autograd.grad(gated_feed_forward(*t), x, torch.ones_like(x, requires_grad=True), create_graph=True)
     with pytest.raises(RuntimeError):  # (once differentiable)
         gx.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [5, 12])
+def test_offsets_beyond_32_bits(rows, dtype):
+    """Rows of x 2^28 values apart."""
+    from crystalformer_b200 import ops
+    tensors, gy = make(rows, 64, 96, dtype)
+    far = torch.zeros((rows - 1) * 2 ** 28 + 64, dtype=dtype, device="cuda")
+    x = far.as_strided((rows, 64), (2 ** 28, 1))
+    x.copy_(tensors[0])
+    assert torch.equal(ops.gated_ffn_fwd(x, *tensors[1:]), ops.gated_ffn_fwd(*tensors))
+    for a, b in zip(ops.gated_ffn_bwd(x, *tensors[1:], "silu", gy), ops.gated_ffn_bwd(*tensors, "silu", gy)):
+        assert torch.equal(a, b)

@@ -259,3 +259,17 @@ def test_refusals():
         QKNorm(8, 16, 9)
     with pytest.raises(ValueError):
         QKNorm(4, 16, 8).cuda()(q, k.repeat(1, 2, 1))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows 2^28 values apart."""
+    from crystalformer_b200 import ops
+    far = torch.zeros(9 * 2 ** 28 + 128, dtype=torch.bfloat16, device="cuda")
+    q, k = far.as_strided((10, 4, 16), (2 ** 28, 16, 1)), far[64:].as_strided((10, 2, 16), (2 ** 28, 16, 1))
+    *_, wq, wk, pos, waves, gq, gk = make(10, 4, 2, 16, 8, 3, 2, "each", torch.bfloat16, 3)
+    q.copy_(torch.randn(q.shape, device="cuda"))
+    k.copy_(torch.randn(k.shape, device="cuda"))
+    for a, b in zip(ops.qk_norm_fwd(q, k, wq, wk, pos, waves), ops.qk_norm_fwd(q.contiguous(), k.contiguous(), wq, wk, pos, waves)):
+        assert torch.equal(a, b)
+    back = lambda q, k: ops.qk_norm_bwd(q, k, wq, wk, pos, waves, 1e-6, False, gq, gk)  # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(back(q, k), back(q.contiguous(), k.contiguous())))
