@@ -254,9 +254,11 @@ std::tuple<Tensor, Tensor> normalize_rotate(const Tensor &q, const Tensor &k, co
                                             const OptTensor &waves, double eps, bool interleaved)
 {
     const Tensor wq = or_none(wq_in), wk = or_none(wk_in);
+    const Tensor place = or_none(pos), cycles = or_none(waves);
+    if (wants_gradients({&place, &cycles})) throw ValueProblem("positions and waves have no gradients here: detach them");
     const variable_list y = wants_gradients({&q, &k, &wq, &wk})
                                 ? NormalizeRotate::apply(q, k, wq_in, wk_in, pos, waves, eps, interleaved)
-                                : qk_norm_fwd(HeadCall(q, k, wq, wk, or_none(pos), or_none(waves), eps, interleaved));
+                                : qk_norm_fwd(HeadCall(q, k, wq, wk, place, cycles, eps, interleaved));
     return {y[0], y[1]};
 }
 

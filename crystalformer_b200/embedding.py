@@ -1,8 +1,8 @@
 """Embedding of species (or any labels) by id: scaled rows of a table, with the gradient of the table from sorted ids.
 
 The reference multiplies one-hot species by the weight of a Linear (models/latticeformer.py:224); the same rows come from a
-lookup, ``embed_species(ids, linear.weight.t())``, which reads the weight where it lies.  ``Latticeformer`` calls it when
-``data.x`` holds species ids instead of one-hot rows."""
+lookup, ``embed_species(ids, linear.weight.t())``, which reads the weight where it lies.  ``Latticeformer`` calls it for a
+batch that holds species ids ``data.z`` instead of one-hot rows ``data.x``."""
 from __future__ import annotations
 
 from torch import Tensor

@@ -21,7 +21,7 @@ def normalize_rotate(q: Tensor, k: Tensor, wq: Optional[Tensor] = None, wk: Opti
     float32, turned: pair p of a head - entries (p, P + p), ``interleaved`` (2p, 2p + 1) - by 2 pi pos . waves[h, p].  Entries from
     2 P on are not turned.  Waves count cycles per unit of position and angles keep their accuracy at any distance.  q and k may
     be strided views (of a joint projection); outputs are contiguous, of their type (float32, bfloat16 or float16).  Gradients: of
-    q, k and the weights."""
+    q, k and the weights; positions and waves that ask for one are refused."""
     return _lib.torch_ops().normalize_rotate(q, k, wq, wk, pos, waves, eps, interleaved)
 
 

@@ -24,6 +24,17 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_positions_and_waves_that_ask_for_gradients_are_refused():
+    """They would get none, and nothing would say so."""
+    from crystalformer_b200.qk_norm import normalize_rotate
+    q, k, pos, waves = torch.zeros(3, 2, 4), torch.zeros(3, 2, 4), torch.zeros(3, 1), torch.zeros(1, 2, 1)
+    for args in ((pos.clone().requires_grad_(), waves), (pos, waves.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="detach"):
+            normalize_rotate(q, k, None, None, *args)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            normalize_rotate(q, k, None, None, *args)
+
+
 def code_of(lib, name, *args):
     with pytest.raises(lib.CrystalformerB200Error) as e:
         lib.call(name, *args)
