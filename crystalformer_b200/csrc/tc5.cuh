@@ -208,10 +208,10 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b,
                  "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
                  : "memory");
 }
-// the barriers at the same place of both blocks
-__device__ __forceinline__ void mma_commit_pair(uint32_t bar)
+// the barriers at the same place of the blocks of `mask`: both, as a rule
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint16_t mask = 3)
 {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask)
                  : "memory");
 }
 

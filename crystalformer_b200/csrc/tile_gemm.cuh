@@ -441,6 +441,11 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                     if (++s == STAGES) { s = 0; phase ^= 1u; }
                 }
             }
+            // every stage given back: a commit arrives in both blocks of a pair, and in neither behind its end
+            for (int i = 0, e = s; i < STAGES && ok; ++i) {
+                ok = mbar_wait(empty(e), e < s ? phase ^ 1u : phase, gave_up);
+                if (++e == STAGES) e = 0;
+            }
             if (!ok && rank == 0) {  // the copies in flight land before the block goes (and its pair: the cluster leaves together)
                 unsigned mine = 0u;
                 for (int i = 0; i < STAGES && i < sent; ++i) {
@@ -545,7 +550,8 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
             }
             if (!ok) {  // the instructions issued so far
                 unsigned mine = 0u;
-                commit(drained);
+                if constexpr (PAIR) mma_commit_pair(drained, 1);  // (here only: the other block has no wait for it)
+                else mma_commit(drained);
                 mbar_wait(drained, 0, &mine);
             }
         }
