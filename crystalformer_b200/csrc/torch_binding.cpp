@@ -2,6 +2,7 @@
 // allocator, the current stream of the tensors' device, and one autograd node each.  Around the C ABI and in C++ because the calls
 // are short: of a training step's 250 us on the host through ctypes and a Python autograd function, 150 were spent outside the library
 // (a backward runs on a thread of autograd's own, where Python code is slow).
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -16,9 +17,10 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
-// What Python gets as TypeError and ValueError; other std::runtime_errors become RuntimeError.
+// What Python gets as TypeError, ValueError and NotImplementedError; other std::runtime_errors become RuntimeError.
 struct TypeProblem : std::runtime_error { using std::runtime_error::runtime_error; };
 struct ValueProblem : std::runtime_error { using std::runtime_error::runtime_error; };
+struct NotThere : std::runtime_error { using std::runtime_error::runtime_error; };
 
 // A C-ABI call that returned a negative status: CrystalformerB200Error in Python.
 struct LibraryError : std::runtime_error {
@@ -90,6 +92,14 @@ variable_list once(variable_list grads)
     return grads;
 }
 
+// A tangent of forward-mode differentiation would end here without a word: outputs are written by address.
+void refuse_tangents(std::initializer_list<const Tensor *> tensors)
+{
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor *t : tensors)
+        if (t->defined() && t->_fw_grad(0).defined()) throw NotThere("the operator has no forward-mode derivative");
+}
+
 bool wants_gradients(std::initializer_list<const Tensor *> tensors)
 {
     if (!at::GradMode::is_enabled()) return false;
@@ -108,6 +118,7 @@ Tensor whole_ids(const Tensor &ids, const Tensor &first)
 
 Tensor embed_fwd(const Tensor &ids_in, const Tensor &table, double scale)
 {
+    refuse_tangents({&table});
     check_first(table, "table", 2);
     const Tensor ids = whole_ids(ids_in, table);
     const int64_t V = table.size(0), D = table.size(1);
@@ -122,6 +133,7 @@ Tensor embed_fwd(const Tensor &ids_in, const Tensor &table, double scale)
 
 Tensor embed_bwd(const Tensor &ids_in, const Tensor &gout, int64_t V, double scale, bool transposed)
 {
+    refuse_tangents({&gout});
     if (gout.dim() < 1) throw ValueProblem("gout must have rows");
     const int64_t D = gout.size(-1), N = ids_in.numel();
     if (gout.sizes().slice(0, gout.dim() - 1) != ids_in.sizes()) throw ValueProblem(text("gout ", gout.sizes(), " does not belong to ids ", ids_in.sizes()));
@@ -155,6 +167,7 @@ struct Embed : torch::autograd::Function<Embed> {
 
 Tensor embed(const Tensor &ids, const Tensor &table, double scale)
 {
+    refuse_tangents({&table});
     return wants_gradients({&table}) ? Embed::apply(table, ids, scale) : embed_fwd(ids, table, scale);
 }
 
@@ -166,6 +179,7 @@ struct HeadCall {
     HeadCall(const Tensor &q_in, const Tensor &k_in, const Tensor &wq_in, const Tensor &wk_in, const Tensor &pos_in, const Tensor &waves_in, double eps,
              bool interleaved)
     {
+        refuse_tangents({&q_in, &k_in, &wq_in, &wk_in, &pos_in, &waves_in});
         check_first(q_in, "q", 3);
         check_first(k_in, "k", 3);
         const int64_t N = q_in.size(0), Hq = q_in.size(1), D = q_in.size(2), Hk = k_in.size(1);
@@ -217,6 +231,7 @@ variable_list qk_norm_fwd(const HeadCall &c)
 
 variable_list qk_norm_bwd(const HeadCall &c, const Tensor &gq_out, const Tensor &gk_out, bool want_wq, bool want_wk)
 {
+    refuse_tangents({&gq_out, &gk_out});
     check_like(gq_out, c.q, "gq_out", c.q.sizes());
     check_like(gk_out, c.q, "gk_out", c.k.sizes());
     const Place place(c.q);
@@ -255,6 +270,7 @@ std::tuple<Tensor, Tensor> normalize_rotate(const Tensor &q, const Tensor &k, co
 {
     const Tensor wq = or_none(wq_in), wk = or_none(wk_in);
     const Tensor place = or_none(pos), cycles = or_none(waves);
+    refuse_tangents({&q, &k, &wq, &wk, &place, &cycles});
     if (wants_gradients({&place, &cycles})) throw ValueProblem("positions and waves have no gradients here: detach them");
     const variable_list y = wants_gradients({&q, &k, &wq, &wk})
                                 ? NormalizeRotate::apply(q, k, wq_in, wk_in, pos, waves, eps, interleaved)
@@ -279,6 +295,7 @@ struct GatedCall {
 
     GatedCall(const Tensor &x, const Tensor &wg, const Tensor &wu, const Tensor &wd, const Tensor &bg, const Tensor &bu, const Tensor &bd, int64_t activation)
     {
+        refuse_tangents({&x, &wg, &wu, &wd, &bg, &bu, &bd});
         check_first(x, "x", 2);
         if (!wg.defined() || !wu.defined() || !wd.defined()) throw TypeProblem("the weights must be tensors");
         if (wg.dim() != 2) throw ValueProblem(text("w_gate must have 2 dimensions, got the shape ", wg.sizes()));
@@ -313,6 +330,7 @@ Tensor gated_fwd(const GatedCall &c)
 
 variable_list gated_bwd(const GatedCall &c, const Tensor &gy_in, const std::array<bool, 7> &wanted)
 {
+    refuse_tangents({&gy_in});
     check_like(gy_in, c.t[0], "gy", c.t[0].sizes());
     const Place place(c.t[0]);
     const Tensor gy = gy_in.contiguous();
@@ -350,6 +368,7 @@ Tensor gated(const Tensor &x_in, const Tensor &wg, const Tensor &wu, const Tenso
              int64_t activation)
 {
     const Tensor bg = or_none(bg_in), bu = or_none(bu_in), bd = or_none(bd_in);
+    refuse_tangents({&x_in, &wg, &wu, &wd, &bg, &bu, &bd});
     const bool rows = x_in.dim() == 2 || x_in.dim() == 0;
     const Tensor x = rows ? x_in : x_in.reshape({-1, x_in.size(-1)});
     const Tensor y = wants_gradients({&x, &wg, &wu, &wd, &bg, &bu, &bd}) ? Gated::apply(x, wg, wu, wd, bg_in, bu_in, bd_in, activation)
@@ -380,6 +399,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
             PyErr_SetString(PyExc_TypeError, e.what());
         } catch (const ValueProblem &e) {
             PyErr_SetString(PyExc_ValueError, e.what());
+        } catch (const NotThere &e) {
+            PyErr_SetString(PyExc_NotImplementedError, e.what());
         }
     });
     using Free = pybind11::call_guard<pybind11::gil_scoped_release>;
