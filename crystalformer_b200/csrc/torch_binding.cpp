@@ -66,9 +66,11 @@ void check_like(const Tensor &t, const Tensor &first, const char *name, at::IntA
 
 void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor or_none(const OptTensor &t) { return t.has_value() ? *t : Tensor(); }
+// What is read by address, negated first where that is still to be done (the imaginary part of a conjugated view).
+Tensor values_of(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
 // the rows of t with their entries as neighbours
-Tensor with_rows(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) != 1 ? t.contiguous() : t; }
-Tensor whole(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+Tensor with_rows(const Tensor &t) { return values_of(t.size(-1) <= 1 || t.stride(-1) != 1 ? t.contiguous() : t); }
+Tensor whole(const Tensor &t) { return t.defined() ? values_of(t.contiguous()) : t; }
 
 struct Place {  // a call's device and stream
     c10::cuda::CUDAGuard guard;
@@ -113,13 +115,14 @@ Tensor whole_ids(const Tensor &ids, const Tensor &first)
 {
     if (ids.device() != first.device()) throw std::runtime_error(text("ids are on ", ids.device(), ", expected ", first.device()));
     if (!at::isIntegralType(ids.scalar_type(), false)) throw TypeProblem(text("ids must be whole numbers, got ", ids.scalar_type()));
-    return ids.to(at::kLong).contiguous();
+    return whole(ids.to(at::kLong));
 }
 
-Tensor embed_fwd(const Tensor &ids_in, const Tensor &table, double scale)
+Tensor embed_fwd(const Tensor &ids_in, const Tensor &table_in, double scale)
 {
-    refuse_tangents({&table});
-    check_first(table, "table", 2);
+    refuse_tangents({&table_in});
+    check_first(table_in, "table", 2);
+    const Tensor table = values_of(table_in);
     const Tensor ids = whole_ids(ids_in, table);
     const int64_t V = table.size(0), D = table.size(1);
     const Place place(table);
@@ -235,7 +238,7 @@ variable_list qk_norm_bwd(const HeadCall &c, const Tensor &gq_out, const Tensor 
     check_like(gq_out, c.q, "gq_out", c.q.sizes());
     check_like(gk_out, c.q, "gk_out", c.k.sizes());
     const Place place(c.q);
-    const Tensor a = gq_out.contiguous(), b = gk_out.contiguous();
+    const Tensor a = whole(gq_out), b = whole(gk_out);
     Tensor gq = at::empty(c.q.sizes(), c.q.options()), gk = at::empty(c.k.sizes(), c.k.options()), gwq, gwk, work;
     if (want_wq && c.wq.defined()) gwq = at::empty(c.wq.sizes(), c.wq.options());
     if (want_wk && c.wk.defined()) gwk = at::empty(c.wk.sizes(), c.wk.options());
@@ -333,7 +336,7 @@ variable_list gated_bwd(const GatedCall &c, const Tensor &gy_in, const std::arra
     refuse_tangents({&gy_in});
     check_like(gy_in, c.t[0], "gy", c.t[0].sizes());
     const Place place(c.t[0]);
-    const Tensor gy = gy_in.contiguous();
+    const Tensor gy = whole(gy_in);
     variable_list grads(7);
     for (int i = 0; i < 7; ++i)
         if (wanted[i] && c.t[i].defined()) grads[i] = at::empty(c.t[i].sizes(), c.t[i].options());
