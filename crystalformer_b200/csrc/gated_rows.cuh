@@ -8,7 +8,8 @@
 // whose 69 MB come in 10.6; 22 by what follows), so products are taken by mma.sync m16n8k16: 16 units by up to eight rows.  The sum does not mind which
 // k an operand calls its own: lane t of a group of four takes eight neighbours, k = 8 t .. 8 t + 7 of each 32, of its two units and of
 // its row, in one 16-byte load each, and both operands of two products are there.  A block's warps share the contraction.  The hidden
-// units go from one kernel to the other as two values of the type, h and what its rounding left, so that only the result is rounded (1 us).
+// units go from one kernel to the other as two values of the type, h and what its rounding left (1 us): 2^-22 of h in float16 and 2^-16
+// in bfloat16 against the result's own rounding, 2^-11 and 2^-8 (float16: 2^-25 at least, half of its smallest number).
 #pragma once
 #include "common.cuh"
 #include "tile_gemm.cuh"
@@ -266,11 +267,11 @@ __global__ void __launch_bounds__(256, 3) hidden_mma_kernel(const __grid_constan
     if (d.b_gate) a += to_float(static_cast<const T *>(d.b_gate)[f]);
     if (d.b_up) b += to_float(static_cast<const T *>(d.b_up)[f]);
     const float v = activation(d.activation, a) * b;
-    const T whole = from_float<T>(v);
-    const float left = v - to_float(whole);
+    // (the largest value stands for all beyond it, and what it leaves carries on: twice the range, then an infinity as by tiles)
+    const float first = to_float(from_float<T>(v)), whole = fabsf(first) <= largest<T>() || first != first ? first : copysignf(largest<T>(), first);
     T *to = h + (long long)r * F + f;
-    to[0] = whole;
-    to[(long long)N * F] = from_float<T>(left == left ? left : 0.f);  // (an infinity leaves none)
+    to[0] = from_float<T>(whole);
+    to[(long long)N * F] = from_float<T>(v - whole);
 }
 
 template <class T>

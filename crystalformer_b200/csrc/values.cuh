@@ -19,6 +19,11 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// the largest finite value
+template <class T> __device__ __forceinline__ float largest();
+template <> __device__ __forceinline__ float largest<__nv_bfloat16>() { return __uint_as_float(0x7f7f0000u); }
+template <> __device__ __forceinline__ float largest<__half>() { return 65504.f; }
+
 // two values of 16 bits in one word, the first in the lower half
 template <class T> __device__ __forceinline__ uint32_t pack_two(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack_two<__nv_bfloat16>(float a, float b)

@@ -22,8 +22,9 @@ def gated_feed_forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, 
     """``(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down`` with the weights of Linears, (F,D), (F,D) and (D,F);
     x (..., D); ``activation``: "silu", "gelu" (the exact one) or "relu".  All of one type; of any sizes.  float32 has float32's
     accuracy (operands in three pieces on the tensor cores); of 16-bit types the hidden features and their gradients are rounded to
-    the type once, sums are float32; float16 has its range too: hidden features beyond 65,504 overflow, and hidden gradients below 6e-5
-    lose digits (scale the loss, as elsewhere in float16).  The backward computes the hidden features again instead of keeping them."""
+    the type once (forward of up to eight rows: not at all, or to twice its digits), sums are float32; float16 has its range too: hidden
+    features beyond 65,504 overflow (of up to eight rows: beyond 131,008 at the earliest), and hidden gradients below 6e-5 lose digits
+    (scale the loss, as elsewhere in float16).  The backward computes the hidden features again instead of keeping them."""
     return _lib.torch_ops().gated(x, w_gate, w_up, w_down, b_gate, b_up, b_down, ops.gate_code(activation))
 
 

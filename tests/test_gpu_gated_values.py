@@ -1,7 +1,7 @@
 """Gated feed-forward block: values at the ends of their types, long contractions, many short launches in a row."""
 import pytest
 import torch
-from test_gpu_gated import TYPES, make
+from test_gpu_gated import TYPES, make, step
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +17,35 @@ def test_short_launches_in_a_row(dtype):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for r in rest for a, b in zip(first, r))
     ops.check_waits()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("on_16_bytes", [True, False])
+@pytest.mark.parametrize("rows", [4, 8, 9])
+def test_hidden_units_at_the_end_of_the_range(rows, on_16_bytes, dtype):
+    """One hidden unit of a value near float16's largest and beyond it (and, in both types, an ordinary one and a small one): nothing but an
+    overflow gives an infinity, and nothing gives what is no number."""
+    from crystalformer_b200.feedforward import gated_feed_forward
+    D, F = (8, 16) if on_16_bytes else (9, 17)
+    zeros = lambda *s: torch.zeros(s, dtype=dtype, device="cuda")  # noqa: E731
+    x, w_gate, w_up, w_down, b_gate = zeros(rows, D), zeros(F, D), zeros(F, D), zeros(D, F), zeros(F) + 1
+    x[:, 0], x[:, 1] = 2, 1
+    w_down[:] = 0.25
+    values = [(0, 1e-5), (0, 0.3), (2.5, 0.125)]
+    if dtype == torch.float16:
+        values += [(32752, 15), (32752, 16), (32752, 17), (-32752, -17), (32752, 4496), (-32752, -4496), (65504, -8), (65504, 30000), (float("inf"), 0)]
+    for pair in values:
+        w_up[3, 0], w_up[3, 1] = pair
+        h = 2 * float(w_up[3, 0]) + float(w_up[3, 1])  # (a product and a sum that are exact in float32)
+        y = gated_feed_forward(x, w_gate, w_up, w_down, b_gate, activation="relu").double()
+        largest = torch.finfo(dtype).max * (1 + 2.0 ** -12)  # (from here on, half a step behind the largest, values round to an infinity)
+        limit = float("inf") if not on_16_bytes and rows <= 8 else 2 * largest - 32 if rows <= 8 else largest
+        if abs(h) >= limit:
+            assert (y == float("inf") * (1 if h > 0 else -1)).all(), (pair, y[0, 0])
+            continue
+        # h in one value of the type, two, or one of float32; then the result.  (What is left of h beyond the largest value, 16 off at
+        # most, is 2^-12 of it.)
+        held = step(dtype) if rows > 8 else 2.0 ** -12 if abs(h) > 65504 else step(dtype) ** 2
+        small = torch.finfo(dtype).smallest_normal * step(dtype) * 2
+        bound = 0.25 * (held * abs(h) + small) + 2 * step(dtype) * abs(0.25 * h) * 0.5 + small
+        assert ((y - 0.25 * h).abs() <= bound * (1 + step(dtype))).all(), (pair, y[0, 0])
