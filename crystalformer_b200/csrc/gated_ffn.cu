@@ -122,7 +122,7 @@ __device__ __forceinline__ void sum_columns(const ColumnJob &job, int block)
         }
     }
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) part[warp][e * 32 + lane] = sum[e] + low[e];
+    for (int e = 0; e < VEC; ++e) part[warp][e * 32 + lane] = fabsf(sum[e]) < INFINITY ? sum[e] + low[e] : sum[e];  // (an infinity loses nothing)
     __syncthreads();
     for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
         const int at = (group * 32 + (i & 31)) * VEC + (i >> 5);

@@ -49,3 +49,27 @@ def test_hidden_units_at_the_end_of_the_range(rows, on_16_bytes, dtype):
         small = torch.finfo(dtype).smallest_normal * step(dtype) * 2
         bound = 0.25 * (held * abs(h) + small) + 2 * step(dtype) * abs(0.25 * h) * 0.5 + small
         assert ((y - 0.25 * h).abs() <= bound * (1 + step(dtype))).all(), (pair, y[0, 0])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 40, 5000])
+@pytest.mark.parametrize("D", [16, 33])
+def test_infinite_gradients_of_biases(D, rows, dtype):
+    """Sums of columns with infinities of one sign, of both, and with what is no number; the other columns stay as they are."""
+    from crystalformer_b200 import ops
+    tensors, gy = make(rows, D, 24, dtype)
+    bias_of = lambda: ops.gated_ffn_bwd(*tensors, "silu", gy, [False] * 6 + [True])[6]  # noqa: E731
+    before = bias_of()
+    inf = float("inf")
+    gy[rows // 2, 1], gy[0, 3], gy[rows - 1, 3] = inf, -inf, -inf
+    gy[0, 5], gy[rows - 1, 5], gy[1, 8] = inf, -inf, float("nan")
+    gb = bias_of()
+    keep = torch.ones(D, dtype=torch.bool, device="cuda")
+    keep[[1, 3, 5, 8]] = False
+    assert gb[1] == inf and gb[3] == -inf and gb[5].isnan() and gb[8].isnan() and torch.equal(gb[keep], before[keep])
+    # dg and du with an infinity: positive inputs and weights, so that nothing cancels (float32: see the values at the ends of its range)
+    positive, one = [t.abs() + 0.1 for t in tensors], torch.ones_like(gy)
+    one[2] = inf
+    gb_gate, gb_up = ops.gated_ffn_bwd(*positive, "relu", one, [False] * 4 + [True, True, False])[4:6]
+    if dtype != torch.float32:
+        assert (gb_gate == inf).all() and (gb_up == inf).all()
