@@ -188,9 +188,9 @@ __device__ __forceinline__ void mma_32(float (&c)[4], const uint4 &lo, const uin
     mma_16x8x16<T>(c, lo.z, hi.z, lo.w, hi.w, x.z, x.w);
 }
 
-// MATS matrices of (M, K) weights by up to eight rows x (ld) of K values: sums[mat][unit of 16][row of 8] of the block's 16 units in
-// `part`, (warps, MATS, 16, 8).  MMA_AHEAD: steps of 32 on their way.  WAIT: x comes from the kernel before (the weights are the
-// caller's, and are fetched earlier).  PIECES: x is the sum of so many matrices, `apart` values apart.
+// MATS matrices of (M, K) weights by up to eight rows x (ld) of K values: sums[mat][piece][unit of 16][row of 8] of the block's 16 units
+// in `part`, (warps, MATS, PIECES, 16, 8).  MMA_AHEAD: steps of 32 on their way.  WAIT: x comes from the kernel before (the weights are
+// the caller's, and are fetched earlier).  PIECES: x is the sum of so many matrices, `apart` values apart, whose sums are kept apart too.
 template <class T, int MATS, int MMA_AHEAD, int PIECES, bool WAIT>
 __device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int K, const T *x, long long ld, long long apart, int rows, int unit0, int warps,
                                            float *part)
@@ -213,11 +213,13 @@ __device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int
 #pragma unroll
     for (int i = 0; i < MMA_AHEAD; ++i) fetch(i, k0 + i * step);
     if constexpr (WAIT) grid_dependency_wait();
-    float c[MATS][4];
+    float c[MATS][PIECES][4];
 #pragma unroll
     for (int m = 0; m < MATS; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c[m][i] = 0.f;
+        for (int q = 0; q < PIECES; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[m][q][i] = 0.f;
     for (int k = k0; k < K; k += MMA_AHEAD * step) {
         uint4 b[MMA_AHEAD][PIECES];
 #pragma unroll
@@ -235,16 +237,18 @@ __device__ __forceinline__ void weigh_rows(const T *const (&w)[MATS], int M, int
 #pragma unroll
             for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                for (int q = PIECES - 1; q >= 0; --q) mma_32<T>(c[m], a[i][m][0], a[i][m][1], b[i][q]);
+                for (int q = 0; q < PIECES; ++q) mma_32<T>(c[m][q], a[i][m][0], a[i][m][1], b[i][q]);
             fetch(i, at + MMA_AHEAD * step);
         }
     }
 #pragma unroll
-    for (int m = 0; m < MATS; ++m) {
-        float *to = part + ((warp * MATS + m) * 16 + g) * 8 + 2 * t;
-        to[0] = c[m][0]; to[1] = c[m][1];
-        to[64] = c[m][2]; to[65] = c[m][3];
-    }
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int q = 0; q < PIECES; ++q) {
+            float *to = part + (((warp * MATS + m) * PIECES + q) * 16 + g) * 8 + 2 * t;
+            to[0] = c[m][q][0]; to[1] = c[m][q][1];
+            to[64] = c[m][q][2]; to[65] = c[m][q][3];
+        }
     __syncthreads();
 }
 
@@ -277,16 +281,20 @@ __global__ void __launch_bounds__(256, 3) hidden_mma_kernel(const __grid_constan
 template <class T>
 __global__ void __launch_bounds__(512) output_mma_kernel(const __grid_constant__ cf_gated_ffn d, const T *h, T *y)
 {
-    __shared__ float part[16 * 128];
+    __shared__ float part[16 * 2 * 128];
     grid_launch_dependents();
     const int unit0 = blockIdx.x * 16, D = (int)d.D, N = (int)d.N;
     const T *const w[1] = {static_cast<const T *>(d.w_down)};
     weigh_rows<T, 1, 6, 2, true>(w, D, (int)d.F, h, d.F, (long long)N * d.F, N, unit0, 16, part);
     const int c = unit0 + (threadIdx.x & 15), r = threadIdx.x >> 4;
     if (r >= N || c >= D) return;
-    float a = 0.f;
+    float a = 0.f, left = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) a += part[(i * 16 + (threadIdx.x & 15)) * 8 + r];
+    for (int i = 0; i < 16; ++i) {
+        a += part[(i * 2 * 16 + (threadIdx.x & 15)) * 8 + r];
+        left += part[((i * 2 + 1) * 16 + (threadIdx.x & 15)) * 8 + r];
+    }
+    if (fabsf(a) < INFINITY) a += left;  // (of an infinite weight what was left of h, zero or of the other sign, says nothing)
     if (d.b_down) a += to_float(static_cast<const T *>(d.b_down)[c]);
     y[(long long)r * D + c] = from_float<T>(a);
 }

@@ -73,3 +73,15 @@ def test_infinite_gradients_of_biases(D, rows, dtype):
     gb_gate, gb_up = ops.gated_ffn_bwd(*positive, "relu", one, [False] * 4 + [True, True, False])[4:6]
     if dtype != torch.float32:
         assert (gb_gate == inf).all() and (gb_up == inf).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_infinite_weights_and_few_rows(dtype):
+    """Rows whose hidden units are handed on in two values: what was left of a unit does not meet an infinite weight."""
+    from crystalformer_b200 import ops
+    tensors, _ = make(3, 16, 24, dtype)
+    tensors = [t.abs() + 0.1 for t in tensors]
+    for value in (float("inf"), -float("inf")):
+        tensors[3][3, 7] = value
+        y = ops.gated_ffn_fwd(*tensors, activation="relu")
+        assert (y[:, 3] == value).all() and y[:, :3].isfinite().all() and y[:, 4:].isfinite().all()
