@@ -69,16 +69,11 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJ
             for (int i = 0; i < 8; ++i) v[i] = i < room ? to_float(src[row * job.ld + col + i]) : 0.f;
         }
         uint32_t w[NP][4];
+        if constexpr (NP == 3) {
+            split_words(v, w);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (NP == 3) {
-                uint32_t s[3];
-                split_words(v[2 * i], v[2 * i + 1], s);
-#pragma unroll
-                for (int q = 0; q < 3; ++q) w[q][i] = s[q];
-            } else {
-                w[0][i] = pack_two<P>(v[2 * i], v[2 * i + 1]);
-            }
+            for (int i = 0; i < 4; ++i) w[0][i] = pack_two<P>(v[2 * i], v[2 * i + 1]);
         }
 #pragma unroll
         for (int q = 0; q < NP; ++q)

@@ -15,12 +15,14 @@
 // the 512 columns, has two of dh alone and computes the next tile's dh beside the epilogue.
 //
 // 16-bit types: one product per pair of blocks; rows of 64 values are 128 bytes.  float32: an operand is the sum of three bfloat16
-// pieces (24 bits, any exponent), made once by a packing kernel or by the epilogue that produces it, and a product is six: piece 0
-// with 0, 1, 2, piece 1 with 0, 1 and piece 2 with 0 (what is left out is 2^-26 of a product).  The tensor core's running sums lose
-// low bits with every instruction, so that with three pieces each block of 64 has accumulators of its own, smallest products first,
-// and the sums over blocks are added in registers: errors are those of float32 sums (3e-7 relative at 512 terms).  The projections of
-// models of up to 128 features, two blocks, stay in their accumulators, the small products of both before the large ones: the
-// epilogue then takes a tile at once, beside the next one's products (backward of 133,120 rows, 128 x 512: 602 -> 455 us).
+// pieces (24 bits of values from 2^-109 on, of smaller ones what lies above 2^-133), made once by a packing kernel or by the epilogue
+// that produces it, and a product is six: piece 0 with 0, 1, 2, piece 1 with 0, 1 and piece 2 with 0 (what is left out is 2^-26 of a
+// product).  What overflows is an infinity, or no number where it meets a value beyond 256, whose second piece may have the other sign.
+// The tensor core's running sums lose low bits with every instruction, so that with three pieces each block of 64 has accumulators of
+// its own, smallest products first, and the sums over blocks are added in registers: errors are those of float32 sums (3e-7 relative at
+// 512 terms).  The projections of models of up to 128 features, two blocks, stay in their accumulators, the small products of both
+// before the large ones: the epilogue then takes a tile at once, beside the next one's products (backward of 133,120 rows, 128 x 512:
+// 602 -> 455 us).
 //
 // All waits are bounded (tc5::mbar_wait); one that runs out ends the block after its copies and products in flight.
 #pragma once
@@ -127,15 +129,29 @@ __device__ __forceinline__ Gate gate_of(float g)
     }
 }
 
-// The three bfloat16 pieces of two values, as words.
-__device__ __forceinline__ void split_words(float a, float b, uint32_t (&w)[3])
+// Two values in one word, the first in the lower half; what would round to an infinity, infinities too, is the largest finite value.
+__device__ __forceinline__ uint32_t pack_two_finite(float a, float b)
+{
+    uint32_t w;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
+    return w;
+}
+
+// The three bfloat16 pieces of 2 COUNT values, as words of two.  The first two are finite: the largest floats keep all their bits, and
+// an infinity is in the third piece, which meets first pieces only - a first piece would meet zeros and pieces of either sign.
+template <int COUNT>
+__device__ __forceinline__ void split_words(const float (&v)[2 * COUNT], uint32_t (&w)[3][COUNT])
 {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        w[i] = pack_two<__nv_bfloat16>(a, b);
-        const float2 f = unpack_two<__nv_bfloat16>(w[i]);
-        a -= f.x;
-        b -= f.y;
+    for (int i = 0; i < COUNT; ++i) {
+        float a = v[2 * i], b = v[2 * i + 1];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            w[p][i] = p < 2 ? pack_two_finite(a, b) : pack_two<__nv_bfloat16>(a, b);
+            const float2 f = unpack_two<__nv_bfloat16>(w[p][i]);
+            a -= f.x;
+            b -= f.y;
+        }
     }
 }
 
@@ -147,16 +163,11 @@ __device__ __forceinline__ void store_planes(const Planes &to, long long row, in
     using P = typename Piece<T>::type;
     P *at = static_cast<P *>(to.base) + row * to.ld + col;
     uint32_t w[NP][8];
+    if constexpr (NP == 3) {
+        split_words(v, w);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (NP == 3) {
-            uint32_t s[3];
-            split_words(v[2 * i], v[2 * i + 1], s);
-#pragma unroll
-            for (int p = 0; p < 3; ++p) w[p][i] = s[p];
-        } else {
-            w[0][i] = pack_two<P>(v[2 * i], v[2 * i + 1]);
-        }
+        for (int i = 0; i < 8; ++i) w[0][i] = pack_two<P>(v[2 * i], v[2 * i + 1]);
     }
 #pragma unroll
     for (int p = 0; p < NP; ++p) store_32(at + p * to.plane, w[p]);

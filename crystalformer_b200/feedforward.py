@@ -21,7 +21,8 @@ def gated_feed_forward(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, 
                        b_down: Optional[Tensor] = None, activation: str = "silu") -> Tensor:
     """``(act(x w_gate^T + b_gate) * (x w_up^T + b_up)) w_down^T + b_down`` with the weights of Linears, (F,D), (F,D) and (D,F);
     x (..., D); ``activation``: "silu", "gelu" (the exact one) or "relu".  All of one type; of any sizes.  float32 has float32's
-    accuracy (operands in three pieces on the tensor cores); of 16-bit types the hidden features and their gradients are rounded to
+    accuracy (operands in three pieces on the tensor cores, which hold values down to 1e-33 whole; infinities, and sums beyond the range,
+    may come out as NaN where they meet values beyond 256); of 16-bit types the hidden features and their gradients are rounded to
     the type once (forward of up to eight rows: not at all, or to twice its digits), sums are float32; float16 has its range too: hidden
     features beyond 65,504 overflow (of up to eight rows: beyond 131,008 at the earliest), and hidden gradients below 6e-5 lose digits
     (scale the loss, as elsewhere in float16).  The backward computes the hidden features again instead of keeping them."""

@@ -1,7 +1,7 @@
 """Gated feed-forward block: values at the ends of their types, long contractions, many short launches in a row."""
 import pytest
 import torch
-from test_gpu_gated import TYPES, make, step
+from test_gpu_gated import TYPES, compare, make, reference, step
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,68 @@ def test_infinite_weights_and_few_rows(dtype):
         tensors[3][3, 7] = value
         y = ops.gated_ffn_fwd(*tensors, activation="relu")
         assert (y[:, 3] == value).all() and y[:, :3].isfinite().all() and y[:, 4:].isfinite().all()
+
+
+def plain(x, w_gate, w_up, w_down, b_gate, b_up, b_down):
+    """With a ReLU, which has a value and a slope at infinity."""
+    linear = torch.nn.functional.linear
+    return linear(torch.relu(linear(x, w_gate, b_gate)) * linear(x, w_up, b_up), w_down, b_down)
+
+
+@pytest.mark.parametrize("rows", [3, 12, 300])
+def test_largest_floats(rows):
+    """Finite values that round to an infinity in bfloat16, as a mask's lowest value is: the same bounds as of any others."""
+    from crystalformer_b200 import ops
+    for sign in (1, -1):
+        tensors, _ = make(rows, 16, 24, torch.float32)
+        x, w_gate, w_up, w_down = tensors[:4]
+        w_gate[:, 0], w_up[:, 0] = 2.0 ** -10 * (1 + torch.linspace(0, 1, 24, device="cuda")), 0.0
+        x[1, 0] = sign * torch.finfo(torch.float32).max
+        want = reference(*tensors, torch.zeros_like(x), "relu")["y"]
+        compare("y", ops.gated_ffn_fwd(*tensors, activation="relu"), want, torch.float32)
+        assert (want[0][1].abs().max() > 1e34) == (sign > 0)
+        # ... and among the weights
+        w_down[3, 5] = sign * torch.finfo(torch.float32).max
+        x[1, 0] = 0.0
+        x *= 0.1
+        want = reference(*tensors, torch.zeros_like(x), "relu")["y"]
+        assert want[0].abs().max() < torch.finfo(torch.float32).max
+        compare("y", ops.gated_ffn_fwd(*tensors, activation="relu"), want, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [3, 12, 300])
+def test_infinities(rows, dtype):
+    """An infinity among the inputs, the weights and the incoming gradient: infinities and what is no number where the formulas have them."""
+    from crystalformer_b200 import ops
+    inf = float("inf")
+    tensors, gy = make(rows, 16, 24, dtype)
+    positive = [t.abs() + 0.1 for t in tensors]  # (so that nothing is inf - inf by itself)
+    for i, at, value in ((0, (1, 0), inf), (0, (1, 0), -inf), (1, (5, 2), inf), (2, (5, 2), -inf), (3, (3, 7), -inf), (0, (2, 4), float("nan"))):
+        t = [v.clone() for v in positive]
+        t[i][at] = value
+        y, want = ops.gated_ffn_fwd(*t, activation="relu"), plain(*(v.double() for v in t))
+        assert torch.equal(y.isnan(), want.isnan()) and torch.equal(y.isinf(), want.isinf()) and torch.equal(y[want.isinf()].double(), want[want.isinf()]), (i, value)
+        assert not want.isfinite().all()
+    one = gy.abs() + 0.1
+    one[2, 3] = inf
+    leaves = [v.double().requires_grad_() for v in positive]
+    want = torch.autograd.grad(plain(*leaves), leaves, one.double())
+    for n, a, b in zip(range(7), ops.gated_ffn_bwd(*positive, "relu", one), want):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.isinf(), b.isinf()) and b.isinf().any(), n
+
+
+def test_smallest_floats():
+    """Three pieces of bfloat16 end at 2^-133: from there on digits are lost, half of that number of a value at most."""
+    from crystalformer_b200 import ops
+    N, D, F = 12, 16, 24
+    tensors, _ = make(N, D, F, torch.float32, bias=False)
+    for scale in (1e-30, 1e-33, 1e-36, 1e-38):
+        x, w_gate, w_up, w_down = tensors[0] * scale, torch.zeros_like(tensors[1]), tensors[2], tensors[3]
+        t = [x, w_gate, w_up, w_down, torch.ones(F, device="cuda"), None, None]
+        y = ops.gated_ffn_fwd(*t, activation="relu")
+        h = x.double() @ w_up.double().t()
+        ref = h @ w_down.double().t()
+        lost = 2.0 ** -134 * (w_up.double().abs().sum(1)[None] + 1) + 2.0 ** -148  # of h: of the values of x, then of itself; of float32 sums
+        bound = reference(*t, torch.zeros_like(x), "relu")["y"][1] + (lost * 2) @ w_down.double().abs().t() + 2.0 ** -148 * F
+        assert ((y.double() - ref).abs() <= bound).all(), scale
