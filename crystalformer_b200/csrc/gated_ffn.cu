@@ -282,6 +282,11 @@ struct Linear {
 //   133,120 rows, 128 x 512, float32                       163; 669              108; 450            157; 756
 //   8,192 rows, 1024 x 2816, bfloat16                       50; 216               84; 355            133; 708
 // (single blocks of 128 x 128 were within 5 % of one of them everywhere).
+//
+// 16-bit types: a share stays in its accumulators from end to end, which lose 1.0e-7 of a sum of one sign with every instruction (the
+// gradient of w_down of 131,072 rows, 8,192 instructions, float16: 8.4e-4 too small, 1.7 times half a step of the type).  So no share is longer
+// than LONGEST: 1,024 instructions, a fifth of half a step of float16.
+constexpr int LONGEST = 256;
 struct Size {
     long long M;
     int N, blocks;
@@ -307,7 +312,7 @@ Cut find_cut(const Size *sizes, int count)
     for (const Kind &k : kinds) {
         const int tm = k.pair ? 2 * TM : TM;
         const double at_once = k.pair ? std::floor(sms / 2) : sms, block = wide ? k.six : k.one;
-        for (int length = most; length >= 1; length = length > 4 ? length * 3 / 4 : length - 1) {
+        for (int length = wide ? most : std::min(most, LONGEST); length >= 1; length = length > 4 ? length * 3 / 4 : length - 1) {
             Cut c{k.tn, k.pair, {}, 0, 0};
             double tiles = 0, work = 0, longest = 0;
             for (int i = 0; i < count; ++i) {

@@ -14,7 +14,8 @@
 // tile's epilogue runs beside the next one's products: two sets of accumulators; GLU_BACKWARD of 16-bit types, whose set is 384 of
 // the 512 columns, has two of dh alone and computes the next tile's dh beside the epilogue.
 //
-// 16-bit types: one product per pair of blocks; rows of 64 values are 128 bytes.  float32: an operand is the sum of three bfloat16
+// 16-bit types: one product per pair of blocks; rows of 64 values are 128 bytes; a contraction stays in its accumulator, in shares short
+// enough for what that loses (find_cut).  float32: an operand is the sum of three bfloat16
 // pieces (24 bits of values from 2^-109 on, of smaller ones what lies above 2^-133), made once by a packing kernel or by the epilogue
 // that produces it, and a product is six: piece 0 with 0, 1, 2, piece 1 with 0, 1 and piece 2 with 0 (what is left out is 2^-26 of a
 // product).  What overflows is an infinity, or no number where it meets a value beyond 256, whose second piece may have the other sign.
