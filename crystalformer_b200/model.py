@@ -52,7 +52,7 @@ def check_batch(data, atoms: int) -> None:
     x, pos, trans, sizes = species_of(data), data.pos, data.trans_vec, data.sizes
     if x.device != pos.device or trans.device != pos.device:
         raise RuntimeError(f"x, pos and trans_vec must be on one device, not on {x.device}, {pos.device} and {trans.device}")
-    if x.dim() != (2 if x.is_floating_point() else 1) or sizes.dim() != 1 or x.shape[0] < atoms or pos.numel() < 3 * atoms or trans.numel() < 9 * sizes.shape[0]:
+    if x.dim() != (1 if getattr(data, "x", None) is None else 2) or sizes.dim() != 1 or x.shape[0] < atoms or pos.numel() < 3 * atoms or trans.numel() < 9 * sizes.shape[0]:
         raise ValueError(f"x {tuple(x.shape)}, pos {tuple(pos.shape)}, trans_vec {tuple(trans.shape)} and sizes {tuple(sizes.shape)} do not "
                          f"hold a batch of {atoms} atoms")
 
