@@ -90,10 +90,14 @@ def image_pointer(image: Optional[Tensor]) -> int:
 
 
 class BatchGeometry:
-    """Everything the attention layers need besides the atom features, computed once per batch on the device."""
+    """Everything the attention layers need besides the atom features, computed once per batch on the device.
+
+    All of it belongs to ``pos`` and ``trans`` as they are at this point of the current stream, whatever is written to them later.
+    ``with_fractional``: True, the fractional coordinates are computed with the rest; False, there are none; None, copies of ``pos`` and
+    ``trans`` are kept to compute them from when they are asked for."""
 
     def __init__(self, pos: Tensor, trans: Tensor, sizes: Tensor, num_atoms: Optional[int] = None,
-                 num_edges: Optional[int] = None, max_atoms: Optional[int] = None):
+                 num_edges: Optional[int] = None, max_atoms: Optional[int] = None, with_fractional: Optional[bool] = None):
         sizes = sizes.to(device=pos.device, dtype=torch.int64)
         if num_atoms is None or num_edges is None or max_atoms is None:
             host = sizes.tolist()  # the one device->host read per batch (the reference does the same, :201)
@@ -105,7 +109,9 @@ class BatchGeometry:
         self.batch, self.edges, self.row_start = prep["batch"], prep["edges"], prep["row_start"]
         self.pos_ij, self.rvecs, self.vcell, self.rvlen = prep["pos_ij"], prep["rvecs"], prep["vcell"], prep["rvlen"]
         self.sizes, self.max_atoms = sizes, int(max_atoms)
-        self._pos, self._trans, self._fractional = pos, trans, None
+        self._moving = pos.requires_grad or trans.requires_grad
+        self._fractional = self._compute_fractional(pos, trans) if with_fractional else None
+        self._cells = (pos.detach().clone(), trans.detach().clone()) if with_fractional is None else None
         self.row_order = ops.row_order(self.atom_start, trans.float(), num_atoms)
         self._kr_base = None
         register_edge_info(self.edges, self.row_start, self.max_atoms, self.row_order)
@@ -119,16 +125,23 @@ class BatchGeometry:
 
     @property
     def fractional(self) -> Tensor:
-        """(N,3) fractional coordinates in [0, 1), built on first use, in 64 bits up to the reduction: a position moved by lattice
-        vectors has the same ones up to the rounding of the position."""
-        if self._fractional is None:
-            pos = self._pos.detach().reshape(-1, 3)[:self.batch.shape[0]].double()
-            t1, t2, t3 = self._trans.detach().reshape(-1, 3, 3).double().unbind(1)
-            rows = torch.stack((torch.linalg.cross(t2, t3), torch.linalg.cross(t3, t1), torch.linalg.cross(t1, t2)), 1)
-            rows = rows / (t1 * rows[:, 0]).sum(1)[:, None, None]
-            f = torch.einsum("nij,nj->ni", rows[self.batch], pos)
-            self._fractional = (f - f.floor()).float()
-        return self._fractional
+        """(N,3) fractional coordinates in [0, 1), in 64 bits up to the reduction: a position moved by lattice vectors has the same ones
+        up to the rounding of the position.  They have no gradient."""
+        if self._fractional is not None:
+            return self._fractional
+        if self._cells is None:
+            raise RuntimeError("this BatchGeometry was built without fractional coordinates: with_fractional=True")
+        return self._compute_fractional(*self._cells)  # (not kept: another stream, or a graph's memory, may be what it is computed in)
+
+    def _compute_fractional(self, pos: Tensor, trans: Tensor) -> Tensor:
+        if self._moving and torch.is_grad_enabled():
+            raise ValueError("positions and lattice vectors have no gradient through the rotation of queries and keys: detach them")
+        pos = pos.detach().reshape(-1, 3)[:self.batch.shape[0]].double()
+        t1, t2, t3 = trans.detach().reshape(-1, 3, 3).double().unbind(1)
+        rows = torch.stack((torch.linalg.cross(t2, t3), torch.linalg.cross(t3, t1), torch.linalg.cross(t1, t2)), 1)
+        rows = rows / (t1 * rows[:, 0]).sum(1)[:, None, None]
+        f = torch.einsum("nij,nj->ni", rows[self.batch], pos)
+        return (f - f.floor()).float()
 
 
 class CrystalformerEncoderLayerCUDA(Module):
@@ -336,19 +349,24 @@ class CrystalformerEncoderCUDA(Module):
         log.extend(zip(pairs[0::2], pairs[1::2]))
         return (ctypes.c_void_p * len(pairs))(*[p.cuda_event for p in pairs])
 
+    def rotates(self) -> bool:
+        """Whether a layer turns its queries and keys by the fractional coordinates."""
+        norms = (getattr(mod.self_attn, "qk_norm", None) for mod in self.layers)
+        return any(norm is not None and norm.waves is not None for norm in norms)
+
     def forward(self, src: Tensor, pos: Tensor, batch: Tensor, trans: Tensor, sizes: Tensor, onehot: Tensor = None,
                 geometry: Optional[BatchGeometry] = None) -> Tensor:
         """Reference signature (…encoder.py:699) plus an optional pre-built ``BatchGeometry``."""
         if src.size(-1) != self.d_model:
             raise RuntimeError("the feature number of src and tgt must be equal to d_model")
-        g = geometry if geometry is not None else BatchGeometry(pos, trans, sizes)
+        rotates = self.rotates()
+        g = geometry if geometry is not None else BatchGeometry(pos, trans, sizes, with_fractional=rotates)
         if self.native and self._native_ok():
             return self._forward_native(src, trans.float().contiguous(), g)
         output = src
+        fractional = g.fractional if rotates else None
         for mod in self.layers:
             kr_base = g.kr_base if mod.domain != "real" else None
-            norm = getattr(mod.self_attn, "qk_norm", None)
-            fractional = g.fractional if norm is not None and norm.waves is not None else None
             output = mod(output, g.batch, g.edges, g.pos_ij, None, trans, kr_base, g.rvecs, g.vcell, onehot, rvlen=g.rvlen,
                          fractional=fractional)
         if self.norm is not None:

@@ -336,7 +336,8 @@ class Latticeformer(nn.Module):
                 return y
         x = self.input_embeddings(species) if onehot else embed_species(species, self.input_embeddings.weight.t())
         if geometry is None:
-            geometry = BatchGeometry(data.pos, data.trans_vec, data.sizes, *(counts if counts is not None else ()))
+            geometry = BatchGeometry(data.pos, data.trans_vec, data.sizes, *(counts if counts is not None else ()),
+                                     with_fractional=self.encoder.rotates())
         g = geometry
         check_batch(data, g.batch.shape[0])
         x = self.encoder(x, data.pos, g.batch, data.trans_vec, g.sizes, geometry=g)
