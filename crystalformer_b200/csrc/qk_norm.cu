@@ -387,10 +387,10 @@ int check_args(const char *who, const cf_qk_norm *d)
     CF_REQUIRE(d, CF_ERR_INVALID, "%s: null pointer", who);
     CF_REQUIRE(known_type(d->type), CF_ERR_UNSUPPORTED, "%s: type %d is none of CF_FLOAT32, CF_BFLOAT16, CF_FLOAT16", who, d->type);
     CF_REQUIRE(d->N >= 0 && d->Hq >= 1 && d->Hk >= 1 && d->D >= 1 && d->P >= 0 && d->C >= 0, CF_ERR_INVALID, "%s: negative size", who);
-    CF_REQUIRE(d->D <= CF_QK_NORM_MAX_DIM && d->Hq <= 1024 && d->N * (d->Hq + d->Hk) < (1ll << 31), CF_ERR_RANGE, "%s: N=%lld Hq=%lld Hk=%lld D=%lld",
+    CF_REQUIRE(d->D <= CF_QK_NORM_MAX_DIM && d->Hq <= 1024 && d->Hk <= 1024 && d->N < (1ll << 31) && d->N * (d->Hq + d->Hk) < (1ll << 31), CF_ERR_RANGE, "%s: N=%lld Hq=%lld Hk=%lld D=%lld",
                who, (long long)d->N, (long long)d->Hq, (long long)d->Hk, (long long)d->D);
     CF_REQUIRE(d->Hq % d->Hk == 0, CF_ERR_INVALID, "%s: %lld query heads do not share %lld key heads evenly", who, (long long)d->Hq, (long long)d->Hk);
-    CF_REQUIRE(2 * d->P <= d->D, CF_ERR_INVALID, "%s: %lld pairs in heads of %lld", who, (long long)d->P, (long long)d->D);
+    CF_REQUIRE(d->P <= d->D / 2, CF_ERR_INVALID, "%s: %lld pairs in heads of %lld", who, (long long)d->P, (long long)d->D);
     CF_REQUIRE(d->q_row < (1ll << 31) && d->q_head < (1ll << 31) && d->k_row < (1ll << 31) && d->k_head < (1ll << 31), CF_ERR_RANGE, "%s: stride of 2^31", who);
     CF_REQUIRE(d->q_row >= 0 && d->q_head >= 0 && d->k_row >= 0 && d->k_head >= 0, CF_ERR_INVALID, "%s: negative stride", who);
     CF_REQUIRE((d->wq_head == 0 || d->wq_head == d->D) && (d->wk_head == 0 || d->wk_head == d->D), CF_ERR_INVALID, "%s: weights are (D) or (H, D)", who);
