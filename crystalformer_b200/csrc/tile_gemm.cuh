@@ -454,10 +454,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                 }
             }
             // every stage given back: a commit arrives in both blocks of a pair, and in neither behind its end
-            for (int i = 0, e = s; i < STAGES && ok; ++i) {
-                ok = mbar_wait(empty(e), e < s ? phase ^ 1u : phase, gave_up);
-                if (++e == STAGES) e = 0;
-            }
+            for (int e = 0; e < STAGES && ok; ++e) ok = mbar_wait(empty(e), e < s ? phase ^ 1u : phase, gave_up);
             if (!ok && rank == 0) {  // the copies in flight land before the block goes (and its pair: the cluster leaves together)
                 unsigned mine = 0u;
                 for (int i = 0; i < STAGES && i < sent; ++i) {
