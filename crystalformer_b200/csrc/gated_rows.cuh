@@ -17,7 +17,12 @@
 
 namespace cf {
 
-constexpr int GATED_ROWS = 8;  // rows up to which this pays against tiles of 128 rows
+// Rows up to which this is taken, eight of mma.sync's columns; tiles take more.  us a call of 4, 8 rows here and of 9, 128 by tiles, one
+// after the other in a graph:
+//   128 x 512, float32        4.3, 6.4; 17.9, 19.6        bfloat16     4.0, 4.1; 12.4, 12.9
+//   2048 x 5632, float32      38.5, 75.8; 142, 143        bfloat16     19.8, 21.0; 35.4, 34.4
+//   2047 x 5631, bfloat16 (off 16 bytes)                               80.4, 74.2; 68.6, 66.2   (one row 36.3)
+constexpr int GATED_ROWS = 8;
 
 namespace rows {
 

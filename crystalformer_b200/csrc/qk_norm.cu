@@ -6,7 +6,8 @@
 //   backward, g' = the output's gradient turned back:  gw_d = sum g'_d x_d r,  gx_d = r (w_d g'_d - x_d r^2 mean_d'(w g' x)).
 //
 // What a pass cannot do without is memory traffic (2 + 2 bytes or 4 + 4 a value forward), but heads are short and 16-bit values many:
-// instruction issue (65 to 70 % of the slots at two blocks per SM) binds it first.  So: an angle is computed once per key head and used
+// 58 to 64 % of the issue slots are taken at two blocks per SM, at 3.6 to 4.7 TB/s.  Neither is used up; each thread has one head on its
+// way while it computes another, 16 KB on an SM in 16 bits, which is less than the bandwidth times the memory's latency.  So: an angle is computed once per key head and used
 // for that key head and the query heads that share it.  A head is held by the fewest lanes (a power of two) that take it in slots of
 // 2 VEC values - a pair of vectors whose entries are partners - so that sums of squares are a few shuffles and nothing is exchanged for
 // the rotation.  A group of lanes walks the rows with the same heads of each: its weights stay in registers, and the next head's values
@@ -387,8 +388,8 @@ int check_args(const char *who, const cf_qk_norm *d)
     CF_REQUIRE(d, CF_ERR_INVALID, "%s: null pointer", who);
     CF_REQUIRE(known_type(d->type), CF_ERR_UNSUPPORTED, "%s: type %d is none of CF_FLOAT32, CF_BFLOAT16, CF_FLOAT16", who, d->type);
     CF_REQUIRE(d->N >= 0 && d->Hq >= 1 && d->Hk >= 1 && d->D >= 1 && d->P >= 0 && d->C >= 0, CF_ERR_INVALID, "%s: negative size", who);
-    CF_REQUIRE(d->D <= CF_QK_NORM_MAX_DIM && d->Hq <= 1024 && d->Hk <= 1024 && d->N < (1ll << 31) && d->N * (d->Hq + d->Hk) < (1ll << 31), CF_ERR_RANGE, "%s: N=%lld Hq=%lld Hk=%lld D=%lld",
-               who, (long long)d->N, (long long)d->Hq, (long long)d->Hk, (long long)d->D);
+    CF_REQUIRE(d->D <= CF_QK_NORM_MAX_DIM && d->Hq <= 1024 && d->Hk <= 1024 && d->N < (1ll << 31) && d->N * (d->Hq + d->Hk) < (1ll << 31),
+               CF_ERR_RANGE, "%s: N=%lld Hq=%lld Hk=%lld D=%lld", who, (long long)d->N, (long long)d->Hq, (long long)d->Hk, (long long)d->D);
     CF_REQUIRE(d->Hq % d->Hk == 0, CF_ERR_INVALID, "%s: %lld query heads do not share %lld key heads evenly", who, (long long)d->Hq, (long long)d->Hk);
     CF_REQUIRE(d->P <= d->D / 2, CF_ERR_INVALID, "%s: %lld pairs in heads of %lld", who, (long long)d->P, (long long)d->D);
     CF_REQUIRE(d->q_row < (1ll << 31) && d->q_head < (1ll << 31) && d->k_row < (1ll << 31) && d->k_head < (1ll << 31), CF_ERR_RANGE, "%s: stride of 2^31", who);

@@ -88,7 +88,7 @@ struct Params {
     float *sums;              // or null: (32 rows each, 2 padded) sums of the columns of dg and du
 };
 constexpr int LINEAR_COUNT = 3;  // products that one launch may have
-constexpr int WHOLE = 2;
+constexpr int WHOLE = 2;  // blocks of a contraction that float32 accumulators keep whole (more of them were not measured)
 template <int MODE> using ParamsOf = Params<MODE == LINEAR ? LINEAR_COUNT : 1>;
 
 template <class T, int MODE, int TN, bool PAIR>
